@@ -19,6 +19,8 @@
  *                           sva/llama.py:330-425 (_inverted_decode_attention)
  *   sva_top_unique          sva/llama.py:83-116 (_top_unique_candidates)
  *   sva_adapter_forward     experiments/sva_late4_logit_distill.py:37-51 (SVAResidualOutputAdapter) + o_proj
+ * Without a reference counterpart: attention over every key (sva_prompt_attention, sva_kv4_*,
+ * sva_cache_evict).
  */
 #ifndef SVA_B200_H_
 #define SVA_B200_H_
@@ -458,6 +460,159 @@ int sva_adapter_forward(const void* hidden, int64_t hidden_row_stride, const voi
                         int32_t dtype, const void* o_weight, const void* o_bias, const float* down, const float* up,
                         float scale, int32_t n_rows, int32_t hidden_dim, int32_t in_dim, int32_t rank, void* out,
                         int64_t out_row_stride, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Attention over every key (no reference counterpart: the reference leaves the prompt and the
+ * unpatched layers to its host framework).  A row that may see no key gets an output of zeros
+ * and a log-sum-exp of -inf.
+ *
+ * sva_prompt_attention: packed sequences.  Sequence b owns query rows [cu_seqlens[b],
+ * cu_seqlens[b + 1]) and key rows [cu_seqlens_k[b], cu_seqlens_k[b + 1]) (device int64, n_seqs + 1
+ * entries; NULL cu_seqlens_k: the same as cu_seqlens).  With Lq query and Lk key rows, query i
+ * sees keys j <= i + Lk - Lq (causal != 0) or all Lk.  Head h reads kv head h / (n_heads /
+ * n_kv_heads).  Strides in elements; rows (head_dim elements) are contiguous.
+ *   out  [n_rows][n_heads][head_dim] by strides; rows outside every sequence are left as they were
+ *   lse  (may be NULL) [n_heads][n_rows] fp32: natural logarithm of the sum of exp(scale q.k)
+ * Boundaries are clamped to the tensors' rows.  head_dim <= 256.  `status` (device int32, may be
+ * NULL) is set to SVA_ERR_TIMEOUT if a bounded wait gave up; the rows concerned become NaN.
+ * ------------------------------------------------------------------------------------- */
+typedef struct sva_prompt_args {
+  int32_t n_seqs, n_heads, n_kv_heads, head_dim;
+  int32_t dtype;  /* sva_dtype of q, keys, values, out */
+  int32_t causal;
+  float softmax_scale;
+  int64_t n_rows, n_key_rows;
+  const void* query;
+  int64_t q_row_stride, q_head_stride;
+  const void* keys;
+  int64_t k_row_stride, k_head_stride;
+  const void* values;
+  int64_t v_row_stride, v_head_stride;
+  const int64_t* cu_seqlens;
+  const int64_t* cu_seqlens_k;
+  void* out;
+  int64_t out_row_stride, out_head_stride;
+  float* lse;
+  int32_t* status;
+} sva_prompt_args;
+
+size_t sva_prompt_attention_workspace_size(const sva_prompt_args* args);
+int sva_prompt_attention(const sva_prompt_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * A key/value cache in 4 bits.  A row of head_dim channels (64 or 128) is head_dim / 2 code
+ * bytes (channel 2j in the low half of byte j, 2j + 1 in the high half) and, for every 32 channels,
+ * a bf16 scale s and a bf16 minimum m; channel value = fma(s, code, m).  Writing a group sets
+ *   m = its smallest value rounded down, s = (its largest value - m) / 15 rounded up (to bf16),
+ *   code = (x - m) / s to the nearest whole number, halves to even (0 where s is 0);
+ * a group holding a NaN or an infinity, or whose range exceeds fp32, reads back as NaN.
+ *   codes  [n_pages][n_kv_heads][page_rows][head_dim / 2] uint8, 16-byte aligned, contiguous
+ *   params [n_pages][n_kv_heads][page_rows][head_dim / 32][2] bf16, 16-byte aligned, contiguous
+ * page_rows is a multiple of 64.  With a page table (int32, one row of page_table_cols pages per
+ * sequence) position l of sequence b is row l % page_rows of page page_table[b][l / page_rows],
+ * page_rows being a power of two; without one it is row l of page b.  Positions outside the cache
+ * (a page number outside [0, n_pages), a row beyond the table) are skipped by writes, read as zeros
+ * and seen by no query.
+ * ------------------------------------------------------------------------------------- */
+typedef struct sva_kv4_cache {
+  int64_t n_pages, page_rows;
+  int32_t n_kv_heads, head_dim;
+  void* k_codes;
+  void* k_params;
+  void* v_codes;
+  void* v_params;
+  const int32_t* page_table;
+  int64_t page_table_stride;
+  int64_t page_table_cols;
+} sva_kv4_cache;
+
+/* Rows of `keys` / `values` (element strides) into the cache.  cu_seqlens NULL: n_tokens rows of
+ * each of n_seqs sequences, token t of sequence b going to position start[b] + t.  Otherwise the
+ * rows are packed (n_tokens in all, seq strides unused) and row n of sequence b goes to position
+ * start[b] + n - cu_seqlens[b]; rows outside every sequence are skipped.  start: device int64 [n_seqs].
+ * Two rows of one call must not meet at one cache row. */
+int sva_kv4_write(const sva_kv4_cache* cache, const void* keys, int64_t k_seq_stride, int64_t k_head_stride,
+                  int64_t k_row_stride, const void* values, int64_t v_seq_stride, int64_t v_head_stride,
+                  int64_t v_row_stride, int32_t dtype, int32_t n_seqs, int64_t n_tokens, const int64_t* start,
+                  const int64_t* cu_seqlens, void* stream);
+
+/* Positions start[b] + t, t < n_tokens, of every sequence back in dtype: keys_out / values_out
+ * [n_seqs][n_kv_heads][n_tokens][head_dim], contiguous. */
+int sva_kv4_read(const sva_kv4_cache* cache, void* keys_out, void* values_out, int32_t dtype, int32_t n_seqs,
+                 int64_t n_tokens, const int64_t* start, void* stream);
+
+/* Attention of each sequence's newest n_tokens tokens over all its cached keys.  Sequence b holds
+ * seq_lens[b] keys (device int64, clamped to [0, max_len]; NULL: max_len); its token t sees keys
+ * [0, seq_lens[b] - n_tokens + t + 1).  Head h reads kv head h / (n_heads / n_kv_heads).
+ *   query / out [n_seqs][n_heads][n_tokens][head_dim] by strides (elements), contiguous rows
+ *   lse     (may be NULL) [n_seqs][n_heads][n_tokens] fp32
+ *   weights (may be NULL) [n_seqs][n_kv_heads][>= max_len] fp32 by strides: the softmax weight of
+ *           every key, summed over the tokens and the heads of its group, is ADDED in place; entries at
+ *           or beyond seq_lens[b] are left as they were.
+ * max_len is at most the cache's capacity (page_rows, or page_table_cols * page_rows) and < 2^31. */
+typedef struct sva_kv4_decode_args {
+  int32_t n_seqs, n_heads, n_tokens, dtype;
+  int64_t max_len;
+  float softmax_scale;
+  const void* query;
+  int64_t q_seq_stride, q_head_stride, q_row_stride;
+  const int64_t* seq_lens;
+  void* out;
+  int64_t out_seq_stride, out_head_stride, out_row_stride;
+  float* lse;
+  float* weights;
+  int64_t weights_seq_stride, weights_head_stride;
+  int32_t* status;
+} sva_kv4_decode_args;
+
+size_t sva_kv4_decode_workspace_size(const sva_kv4_cache* cache, const sva_kv4_decode_args* args);
+int sva_kv4_decode(const sva_kv4_cache* cache, const sva_kv4_decode_args* args, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Eviction from a cache by accumulated attention weight.  For each sequence b and kv head h holding
+ * n = seq_lens[b] rows (device int64, clamped to [0, max_len]): all rows stay if n <= keep, else the last
+ * min(recent, keep) rows and, of the others, those with the largest weights[b][h][l] (ties: the
+ * lowest l; NaN counts as the largest).  The rows that stay move, in ascending order of l, to
+ * positions 0, 1, ... of every row array and of the weights; other rows are left as they were, and
+ * weights behind the rows that stayed become 0 over the whole destination width.
+ *   arrays: up to SVA_EVICT_MAX_ARRAYS of rows of row_bytes bytes (a multiple of 2), rows contiguous per
+ *           [page][head]; dst may equal src (in place), else the two must not overlap.  Page tables
+ *           as for sva_kv4_cache, one for the sources and one for the destinations; NULL: page b.
+ *           No page may belong to two sequences in place.
+ *   kept_out [n_seqs][n_kv_heads][keep] int32 ascending, -1 padded; lens_out [n_seqs] int64 = min(n, keep)
+ * weights [b][h] start at strides (elements); dst_weights may equal weights.  lens_out may be seq_lens.
+ * ------------------------------------------------------------------------------------- */
+#define SVA_EVICT_MAX_ARRAYS 8
+typedef struct sva_evict_array {
+  const void* src;
+  void* dst;
+  int64_t row_bytes;
+  int64_t src_page_stride, src_head_stride; /* bytes */
+  int64_t dst_page_stride, dst_head_stride; /* bytes */
+} sva_evict_array;
+
+typedef struct sva_evict_args {
+  int32_t n_seqs, n_kv_heads, n_arrays;
+  int32_t in_place;
+  int64_t max_len, keep, recent;
+  const int64_t* seq_lens;
+  const float* weights;
+  int64_t weights_seq_stride, weights_head_stride;
+  float* dst_weights;
+  int64_t dst_weights_seq_stride, dst_weights_head_stride, dst_weights_width;
+  int64_t src_pages, src_page_rows, dst_pages, dst_page_rows;
+  const int32_t* src_table;
+  int64_t src_table_stride, src_table_cols;
+  const int32_t* dst_table;
+  int64_t dst_table_stride, dst_table_cols;
+  int32_t* kept_out;
+  int64_t* lens_out;
+} sva_evict_args;
+
+size_t sva_cache_evict_workspace_size(const sva_evict_args* args);
+int sva_cache_evict(const sva_evict_args* args, const sva_evict_array* arrays, void* workspace,
+                    size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -73,6 +73,14 @@ EXPORTED = (
     "sva_inverted_shard_combine",
     "sva_top_unique",
     "sva_adapter_forward",
+    "sva_prompt_attention_workspace_size",
+    "sva_prompt_attention",
+    "sva_kv4_write",
+    "sva_kv4_read",
+    "sva_kv4_decode_workspace_size",
+    "sva_kv4_decode",
+    "sva_cache_evict_workspace_size",
+    "sva_cache_evict",
 )
 
 c_i32 = ctypes.c_int32
@@ -210,6 +218,134 @@ class InvertedArgs(ctypes.Structure):
     ]
 
 
+class PromptArgs(ctypes.Structure):
+    """Mirror of ``sva_prompt_args``."""
+
+    _fields_ = [
+        ("n_seqs", c_i32),
+        ("n_heads", c_i32),
+        ("n_kv_heads", c_i32),
+        ("head_dim", c_i32),
+        ("dtype", c_i32),
+        ("causal", c_i32),
+        ("softmax_scale", c_f32),
+        ("n_rows", c_i64),
+        ("n_key_rows", c_i64),
+        ("query", c_vp),
+        ("q_row_stride", c_i64),
+        ("q_head_stride", c_i64),
+        ("keys", c_vp),
+        ("k_row_stride", c_i64),
+        ("k_head_stride", c_i64),
+        ("values", c_vp),
+        ("v_row_stride", c_i64),
+        ("v_head_stride", c_i64),
+        ("cu_seqlens", c_vp),
+        ("cu_seqlens_k", c_vp),
+        ("out", c_vp),
+        ("out_row_stride", c_i64),
+        ("out_head_stride", c_i64),
+        ("lse", c_vp),
+        ("status", c_vp),
+    ]
+
+
+class Kv4CacheArgs(ctypes.Structure):
+    """Mirror of ``sva_kv4_cache``."""
+
+    _fields_ = [
+        ("n_pages", c_i64),
+        ("page_rows", c_i64),
+        ("n_kv_heads", c_i32),
+        ("head_dim", c_i32),
+        ("k_codes", c_vp),
+        ("k_params", c_vp),
+        ("v_codes", c_vp),
+        ("v_params", c_vp),
+        ("page_table", c_vp),
+        ("page_table_stride", c_i64),
+        ("page_table_cols", c_i64),
+    ]
+
+
+class Kv4DecodeArgs(ctypes.Structure):
+    """Mirror of ``sva_kv4_decode_args``."""
+
+    _fields_ = [
+        ("n_seqs", c_i32),
+        ("n_heads", c_i32),
+        ("n_tokens", c_i32),
+        ("dtype", c_i32),
+        ("max_len", c_i64),
+        ("softmax_scale", c_f32),
+        ("query", c_vp),
+        ("q_seq_stride", c_i64),
+        ("q_head_stride", c_i64),
+        ("q_row_stride", c_i64),
+        ("seq_lens", c_vp),
+        ("out", c_vp),
+        ("out_seq_stride", c_i64),
+        ("out_head_stride", c_i64),
+        ("out_row_stride", c_i64),
+        ("lse", c_vp),
+        ("weights", c_vp),
+        ("weights_seq_stride", c_i64),
+        ("weights_head_stride", c_i64),
+        ("status", c_vp),
+    ]
+
+
+EVICT_MAX_ARRAYS = 8  # SVA_EVICT_MAX_ARRAYS
+
+
+class EvictArray(ctypes.Structure):
+    """Mirror of ``sva_evict_array``."""
+
+    _fields_ = [
+        ("src", c_vp),
+        ("dst", c_vp),
+        ("row_bytes", c_i64),
+        ("src_page_stride", c_i64),
+        ("src_head_stride", c_i64),
+        ("dst_page_stride", c_i64),
+        ("dst_head_stride", c_i64),
+    ]
+
+
+class EvictArgs(ctypes.Structure):
+    """Mirror of ``sva_evict_args``."""
+
+    _fields_ = [
+        ("n_seqs", c_i32),
+        ("n_kv_heads", c_i32),
+        ("n_arrays", c_i32),
+        ("in_place", c_i32),
+        ("max_len", c_i64),
+        ("keep", c_i64),
+        ("recent", c_i64),
+        ("seq_lens", c_vp),
+        ("weights", c_vp),
+        ("weights_seq_stride", c_i64),
+        ("weights_head_stride", c_i64),
+        ("dst_weights", c_vp),
+        ("dst_weights_seq_stride", c_i64),
+        ("dst_weights_head_stride", c_i64),
+        ("dst_weights_width", c_i64),
+        ("src_pages", c_i64),
+        ("src_page_rows", c_i64),
+        ("dst_pages", c_i64),
+        ("dst_page_rows", c_i64),
+        ("src_table", c_vp),
+        ("src_table_stride", c_i64),
+        ("src_table_cols", c_i64),
+        ("dst_table", c_vp),
+        ("dst_table_stride", c_i64),
+        ("dst_table_cols", c_i64),
+        ("kept_out", c_vp),
+        ("lens_out", c_vp),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -275,6 +411,18 @@ def load() -> ctypes.CDLL:
                                 ctypes.POINTER(ctypes.c_int32), c_vp], ctypes.c_int),
             "sva_adapter_forward": ([c_vp, c_i64, c_vp, c_i64, c_i32, c_vp, c_vp, c_vp, c_vp, c_f32, c_i32, c_i32,
                                      c_i32, c_i32, c_vp, c_i64, c_vp], ctypes.c_int),
+            "sva_prompt_attention_workspace_size": ([ctypes.POINTER(PromptArgs)], c_sz),
+            "sva_prompt_attention": ([ctypes.POINTER(PromptArgs), c_vp, c_sz, c_vp], ctypes.c_int),
+            "sva_kv4_write": ([ctypes.POINTER(Kv4CacheArgs), c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64,
+                               c_i32, c_i32, c_i64, c_vp, c_vp, c_vp], ctypes.c_int),
+            "sva_kv4_read": ([ctypes.POINTER(Kv4CacheArgs), c_vp, c_vp, c_i32, c_i32, c_i64, c_vp, c_vp],
+                             ctypes.c_int),
+            "sva_kv4_decode_workspace_size": ([ctypes.POINTER(Kv4CacheArgs), ctypes.POINTER(Kv4DecodeArgs)], c_sz),
+            "sva_kv4_decode": ([ctypes.POINTER(Kv4CacheArgs), ctypes.POINTER(Kv4DecodeArgs), c_vp, c_sz, c_vp],
+                               ctypes.c_int),
+            "sva_cache_evict_workspace_size": ([ctypes.POINTER(EvictArgs)], c_sz),
+            "sva_cache_evict": ([ctypes.POINTER(EvictArgs), ctypes.POINTER(EvictArray), c_vp, c_sz, c_vp],
+                                ctypes.c_int),
         }
         for name, (argtypes, restype) in sigs.items():
             fn = getattr(lib, name, None)

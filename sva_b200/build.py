@@ -15,7 +15,7 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 OUT = HERE / "libsva_b200.so"
-SOURCES = ["capi.cu", "catalog.cu", "decode.cu", "postings.cu", "inverted.cu", "adapter.cu"]
+SOURCES = ["capi.cu", "catalog.cu", "decode.cu", "postings.cu", "inverted.cu", "adapter.cu", "kv4.cu", "evict.cu", "prompt.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

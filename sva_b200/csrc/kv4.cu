@@ -1,0 +1,1000 @@
+// A key/value cache in 4 bits: rows written and read back, and attention of the newest tokens over
+// every cached key.
+//
+// Format.  A row of D channels (64 or 128) is D/2 code bytes and, per group of 32 channels, a bf16
+// scale s and minimum m: value = m + s c, c in 0..15.  m is rounded down and s up, so that all values of
+// the group lie in [m, m + 15 s] and no code has to be clamped.
+#include <type_traits>
+
+#include "async_copy.cuh"
+#include "sva_common.cuh"
+#include "sva_internal.h"
+
+namespace sva {
+
+constexpr int kGroup = 32;
+constexpr int kTileKeys = 64;  // keys of one pipeline stage; page_rows is a multiple of it
+
+struct Kv4 {
+  int64_t n_pages, page_rows;
+  int n_kv, shift;  // page_rows == 1 << shift with a page table
+  uint8_t* k_codes;
+  uint32_t* k_params;
+  uint8_t* v_codes;
+  uint32_t* v_params;
+  const int32_t* table;
+  int64_t table_stride, table_cols;
+
+  // Row index (over [page][row] of kv head h) of position l of sequence b, or -1.
+  __device__ __forceinline__ int64_t row(int b, int h, int64_t l) const {
+    int64_t page = b, r = l;
+    if (l < 0) return -1;
+    if (table) {
+      const int64_t col = l >> shift;
+      if (col >= table_cols) return -1;
+      page = __ldg(table + b * table_stride + col);
+      r = l & (page_rows - 1);
+    }
+    if (page < 0 || page >= n_pages || r >= page_rows) return -1;
+    return (page * n_kv + h) * page_rows + r;
+  }
+};
+
+// ---------------------------------------------------------------------------------------
+// rows in and out
+// ---------------------------------------------------------------------------------------
+// Eight channels a thread, four threads a group: the group's extremes take two shuffles, a thread's
+// eight codes are one 32-bit word.  HBM bound: D * size + D/2 + D/8 bytes a row.
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool vec, float x[8]) {
+  if constexpr (sizeof(T) == 4) {
+    if (vec) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+      return;
+    }
+  } else {
+    if (vec) {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+      const T* e = reinterpret_cast<const T*>(&a);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(e[i]);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(p[i]);
+}
+
+// Code of x: (x - m) / s to the nearest whole number, halves to even.  For 16-bit inputs the fp32
+// quotient decides: x - m and the halves (k + 1/2) s are fp32 numbers, so a quotient that is a half
+// is found as one.  fp32 inputs leave a remainder in x - m, and the two neighbours are compared in 64 bits.
+template <typename T>
+__device__ __forceinline__ uint32_t code_of(float x, float m, float s, float inv) {
+  const float d = x - m;
+  float q = d * inv;
+  q = fmaf(fmaf(-q, s, d), inv, q);
+  float c = rintf(q);
+  if constexpr (sizeof(T) == 4) {
+    if (fabsf(fabsf(q - c) - 0.5f) < 1e-4f) {
+      const double base = floor((double)q), rest = ((double)x - (double)m) - (base + 0.5) * (double)s;
+      const bool odd = (((int)base) & 1) != 0;
+      c = (float)((rest > 0.0 || (rest == 0.0 && odd)) ? base + 1.0 : base);
+    }
+  }
+  return (uint32_t)fminf(fmaxf(c, 0.f), 15.f);
+}
+
+struct Kv4WriteParams {
+  Kv4 c;
+  const void* x[2];
+  int64_t seq_stride[2], head_stride[2], row_stride[2];
+  bool vec[2];
+  int n_seqs;
+  int64_t n_tokens;
+  const int64_t* start;
+  const int64_t* cu;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4WriteParams p) {
+  constexpr int kLanes = D / 8, kRows = 256 / kLanes, kUnroll = 4;
+  const int which = blockIdx.z;
+  const int h = blockIdx.y % p.c.n_kv, lane = threadIdx.x % kLanes;
+  int b = blockIdx.y / p.c.n_kv;
+  const T* base = reinterpret_cast<const T*>(p.x[which]) + h * p.head_stride[which] + lane * 8;
+  if (!p.cu) base += b * p.seq_stride[which];
+  uint8_t* codes = which ? p.c.v_codes : p.c.k_codes;
+  uint32_t* params = which ? p.c.v_params : p.c.k_params;
+  const int64_t t0 = (int64_t)blockIdx.x * (kRows * kUnroll) + threadIdx.x / kLanes;
+  float x[kUnroll][8];
+  int64_t row[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t t = t0 + u * kRows;
+    row[u] = -1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
+    if (t >= p.n_tokens) continue;
+    int64_t l = t;
+    if (p.cu) {
+      // the last sequence that begins at or before t
+      int lo = 0, hi = p.n_seqs;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(p.cu + mid) <= t) lo = mid; else hi = mid;
+      }
+      b = lo;
+      if (__ldg(p.cu + b) > t || __ldg(p.cu + b + 1) <= t) continue;
+      l = t - __ldg(p.cu + b);
+    }
+    row[u] = p.c.row(b, h, __ldg(p.start + b) + l);
+    load8<T>(base + t * p.row_stride[which], p.vec[which], x[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    float low = x[u][0], high = x[u][0];
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      low = fminf(low, x[u][i]);
+      high = fmaxf(high, x[u][i]);
+      sum += x[u][i] * 0.f;  // NaN for a NaN or an infinity
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      low = fminf(low, __shfl_xor_sync(0xFFFFFFFFu, low, o));
+      high = fmaxf(high, __shfl_xor_sync(0xFFFFFFFFu, high, o));
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    }
+    const __nv_bfloat16 mb = __float2bfloat16_rd(low);
+    const float m = __bfloat162float(mb);
+    const __nv_bfloat16 sb = __float2bfloat16_ru(__fdiv_ru(__fsub_ru(high, m), 15.f));
+    const float s = __bfloat162float(sb);
+    const bool bad = !(sum == 0.f) || !(fabsf(m) <= 3.4e38f) || !(s <= 3.4e38f);
+    // scaling by a power of two keeps 1 / s finite for the smallest scales
+    const float lift = s < 1e-30f ? 0x1p100f : 1.f;
+    const float inv = (s > 0.f && !bad) ? 1.f / (s * lift) : 0.f;
+    uint32_t w = 0;
+    if (!bad) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w |= code_of<T>(x[u][i] * lift, m * lift, s * lift, inv) << (4 * i);
+    }
+    if (row[u] >= 0) {
+      reinterpret_cast<uint32_t*>(codes)[row[u] * kLanes + lane] = w;
+      if ((lane & 3) == 0)
+        params[row[u] * (D / kGroup) + (lane >> 2)] =
+            bad ? 0x7FFF7FFFu
+                : ((uint32_t)__bfloat16_as_ushort(mb) << 16) | (uint32_t)__bfloat16_as_ushort(sb);
+    }
+  }
+}
+
+struct Kv4ReadParams {
+  Kv4 c;
+  void* out[2];
+  int64_t n_tokens;
+  const int64_t* start;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
+  constexpr int kLanes = D / 8, kRows = 256 / kLanes, kUnroll = 4;
+  const int which = blockIdx.z;
+  const int h = blockIdx.y % p.c.n_kv, b = blockIdx.y / p.c.n_kv, lane = threadIdx.x % kLanes;
+  const uint32_t* codes = reinterpret_cast<const uint32_t*>(which ? p.c.v_codes : p.c.k_codes);
+  const uint32_t* params = which ? p.c.v_params : p.c.k_params;
+  const int64_t t0 = (int64_t)blockIdx.x * (kRows * kUnroll) + threadIdx.x / kLanes;
+  const int64_t start = __ldg(p.start + b);
+  uint32_t w[kUnroll], sm[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t t = t0 + u * kRows;
+    w[u] = sm[u] = 0;
+    if (t >= p.n_tokens) continue;
+    const int64_t row = p.c.row(b, h, start + t);
+    if (row < 0) continue;
+    w[u] = __ldg(codes + row * kLanes + lane);
+    sm[u] = __ldg(params + row * (D / kGroup) + (lane >> 2));
+  }
+  T* out = reinterpret_cast<T*>(p.out[which]) + (int64_t)blockIdx.y * p.n_tokens * D + lane * 8;
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t t = t0 + u * kRows;
+    if (t >= p.n_tokens) continue;
+    const float s = __uint_as_float(sm[u] << 16), m = __uint_as_float(sm[u] & 0xFFFF0000u);
+    __align__(16) T y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = from_f32<T>(fmaf(s, (float)((w[u] >> (4 * i)) & 15u), m));
+    uint4* dst = reinterpret_cast<uint4*>(out + t * D);
+    dst[0] = reinterpret_cast<const uint4*>(y)[0];
+    if constexpr (sizeof(T) == 4) dst[1] = reinterpret_cast<const uint4*>(y)[1];
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// attention over the cache
+// ---------------------------------------------------------------------------------------
+// One CTA takes a chunk of the keys of one (sequence, kv head) and up to 8 NT query columns (tokens x
+// heads of the group); each of its warps streams its own 64-key tiles through its own ring of bulk
+// copies (no CTA barrier in the loop) and keeps its own running maximum and sum per column.
+//
+// Mathematics.  With centred codes c - 8 (exact in bf16) and centre z = m + 8 s of a key's group g,
+//   q.k    = sum_g s_g (q_g . (c_g - 8)) + z_g sum(q_g)
+//   sum p v = sum_g [ (p s_g) . (c_g - 8) ] + sum_keys p z_g
+// so the tensor cores multiply whole numbers and the scales act on fp32 accumulators: the only
+// roundings are those of q (none: bf16 parts) and of p s to bf16 (one part: 2^-9 of a weight, for
+// 16-bit outputs; three parts, 2^-24 or better, for fp32).
+//
+// Layout.  mma.m16n8k16 with the cache as the 16-row operand and the columns as N: keys x channels for
+// the scores, channels x keys for the output, because a decode step has few columns (heads of a
+// group), for which a 128-row tcgen05 tile would be empty.  Slot r of a 16-key tile is physical key
+// slot_key(r), which makes the value loads of a warp fall into 32 different banks.
+
+constexpr int kDecWarps = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Kv4DecParams {
+  Kv4 c;
+  const void* q;
+  int64_t q_seq, q_head, q_row;
+  void* out;
+  int64_t o_seq, o_head, o_row;
+  const int64_t* seq_lens;
+  int64_t max_len;
+  float scale_log2, scale;
+  int n_heads, n_tokens, groups, n_cols, col_tiles;
+  int n_chunks;
+  int64_t chunk_keys;
+  float* lse;
+  float* weights;
+  int64_t w_seq, w_head;
+  float* part_ml;  // [problem][chunk][8 NT][2]
+  float* part_o;   // [problem][chunk][8 NT][D]
+  float* logits;   // [sequence][kv head][column][logit_stride]
+  int64_t logit_stride;
+  int* status;
+};
+
+__device__ __forceinline__ int64_t seq_len_of(const Kv4DecParams& p, int b) {
+  int64_t n = p.max_len;
+  if (p.seq_lens) {
+    n = __ldg(p.seq_lens + b);
+    n = n < 0 ? 0 : (n > p.max_len ? p.max_len : n);
+  }
+  return n;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+
+__device__ __forceinline__ void mma_bf16(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// 2^x by the hardware's approximation (2 units of 2^-23 relative; results below 2^-126 become 0, which a
+// softmax weight beside a weight of 1 cannot show).
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// Two codes in the low bits of both halves of v -> bf16 pair of code - 8: 0x4300 is 128 with the code
+// as its lowest mantissa bits, 0x4308 is 136.
+__device__ __forceinline__ uint32_t codes_bf16(uint32_t v) {
+  const uint32_t x = (v & 0x000F000Fu) | 0x43004300u;
+  const __nv_bfloat162 d = __hsub2(reinterpret_cast<const __nv_bfloat162&>(x),
+                                   __nv_bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308)));
+  return reinterpret_cast<const uint32_t&>(d);
+}
+
+__device__ __forceinline__ int slot_key(int r) { return (r & 8) + ((r & 7) >> 1) + 4 * (r & 1); }
+
+template <typename T, int D, int NT>
+struct DecShape {
+  static constexpr bool kWide = sizeof(T) == 4;
+  static constexpr int kQParts = kWide ? 3 : (std::is_same<T, __half>::value ? 2 : 1);  // bf16 parts of q: exact
+  static constexpr int kPParts = kWide ? 3 : 1;
+  static constexpr int kGroups = D / kGroup;
+  static constexpr int kTileBytes = kTileKeys * (D / 2 + D / 8) * 2;
+  static constexpr int kStages = D == 64 ? 3 : 2;
+  static constexpr int kCols = 8 * NT;
+  static constexpr int kSmem = kDecWarps * kStages * kTileBytes + 128;
+};
+
+template <typename T, int D, int NT, bool kLogits>
+__global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4DecParams p) {
+  using S = DecShape<T, D, NT>;
+  constexpr int kG = S::kGroups, kStages = S::kStages;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int ct = blockIdx.y % p.col_tiles, h = blockIdx.y / p.col_tiles, b = blockIdx.z;
+  const int chunk = blockIdx.x;
+  const int col0 = ct * S::kCols;
+  const int64_t len = seq_len_of(p, b);
+  const int64_t key0 = chunk * p.chunk_keys, key1 = min(len, key0 + p.chunk_keys);
+  if (key0 >= len && chunk > 0) return;  // the join reads ceil(len / chunk_keys) chunks (at least one)
+
+  unsigned char* ring = smem + 128 + warp * (kStages * S::kTileBytes);
+  const uint32_t bar0 = smem_u32(smem) + warp * (8 * kStages);
+  if (lane == 0) {
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) mbar_init(bar0 + 8 * s, 1);
+    mbar_fence_init();
+  }
+  __syncwarp();
+
+  const int n_tiles = key1 > key0 ? (int)((key1 - key0 + kTileKeys - 1) / kTileKeys) : 0;
+  const int my_tiles = n_tiles > warp ? (n_tiles - warp + kDecWarps - 1) / kDecWarps : 0;
+  // lane i holds the row index of this warp's tile 32 k + i; -1: not in the cache
+  auto rows_of = [&](int it0) -> int64_t {
+    const int i = it0 + lane;
+    return i < my_tiles ? p.c.row(b, h, key0 + (int64_t)(warp + i * kDecWarps) * kTileKeys) : -1;
+  };
+  int64_t rows_cur = rows_of(0), rows_next = rows_of(32);
+  auto issue = [&](int it, int base) {  // copies of tile it into stage it % kStages; base: first tile of rows_cur
+    const int64_t r = it < base + 32 ? __shfl_sync(0xFFFFFFFFu, rows_cur, it - base)
+                                     : __shfl_sync(0xFFFFFFFFu, rows_next, it - base - 32);
+    if (lane == 0) {
+      const int s = it % kStages;
+      const uint32_t bar = bar0 + 8 * s, dst = smem_u32(ring + s * S::kTileBytes);
+      constexpr uint32_t kC = kTileKeys * D / 2, kP = kTileKeys * D / 8;
+      if (r >= 0) {
+        mbar_expect_tx(bar, S::kTileBytes);
+        bulk_load(dst, p.c.k_codes + r * (D / 2), kC, bar);
+        bulk_load(dst + kC, p.c.k_params + r * kG, kP, bar);
+        bulk_load(dst + kC + kP, p.c.v_codes + r * (D / 2), kC, bar);
+        bulk_load(dst + 2 * kC + kP, p.c.v_params + r * kG, kP, bar);
+      } else {
+        mbar_arrive(bar);
+      }
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < kStages; ++s)
+    if (s < my_tiles) issue(s, 0);
+
+  // query fragments: column g of every 8-column tile, channels 32 G + 8 t .. + 7, pairs (i, i + 4)
+  uint32_t qf[kG][S::kQParts][NT][4];
+  float qsum[kG][NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int col = col0 + 8 * n + g;
+    const bool live = col < p.n_cols;
+    const int tok = col / p.groups, head = h * p.groups + col % p.groups;
+    const T* src = reinterpret_cast<const T*>(p.q) + b * p.q_seq + (int64_t)head * p.q_head + (int64_t)tok * p.q_row;
+#pragma unroll
+    for (int gr = 0; gr < kG; ++gr) {
+      float x[8], sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = live ? to_f32<T>(src[gr * kGroup + 8 * t + i]) : 0.f;
+        sum += x[i];
+      }
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+      // this lane accumulates columns 2t and 2t + 1
+      qsum[gr][n][0] = __shfl_sync(0xFFFFFFFFu, sum, (2 * t) * 4);
+      qsum[gr][n][1] = __shfl_sync(0xFFFFFFFFu, sum, (2 * t + 1) * 4);
+#pragma unroll
+      for (int part = 0; part < S::kQParts; ++part) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t v = pack_bf16(x[i], x[i + 4]);
+          qf[gr][part][n][i] = v;
+          x[i] -= bf16_lo(v);
+          x[i + 4] -= bf16_hi(v);
+        }
+      }
+    }
+  }
+  int limit[NT][2];  // keys that columns 2t and 2t + 1 see, counted from key0
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int col = col0 + 8 * n + 2 * t + j;
+      const int64_t seen = len - p.n_tokens + col / p.groups + 1 - key0;
+      limit[n][j] = col < p.n_cols ? (int)min(max(seen, (int64_t)0), p.chunk_keys) : 0;
+    }
+
+  float m_run[NT][2], l_run[NT][2], zsum[kG][NT][2], acc[kG][2][NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) m_run[n][j] = -INFINITY, l_run[n][j] = 0.f;
+#pragma unroll
+  for (int gr = 0; gr < kG; ++gr)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      zsum[gr][n][0] = zsum[gr][n][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[gr][0][n][i] = acc[gr][1][n][i] = 0.f;
+    }
+
+  bool failed = false;
+  int failed_at = 0, base = 0;
+  const int key_a = slot_key(g);
+  for (int it = 0; it < my_tiles; ++it) {
+    if (it == base + 32) {
+      base += 32;
+      rows_cur = rows_next;
+      rows_next = rows_of(base + 32);
+    }
+    const int s = it % kStages;
+    if (!mbar_wait(bar0 + 8 * s, (it / kStages) & 1)) {
+      failed = true;
+      failed_at = it;
+      break;
+    }
+    const bool there = __shfl_sync(0xFFFFFFFFu, rows_cur, it - base) >= 0;
+    const int l0 = (warp + it * kDecWarps) * kTileKeys;  // first key of the tile, counted from key0
+    const unsigned char* kc = ring + s * S::kTileBytes;
+    const unsigned char* kp = kc + kTileKeys * D / 2;
+    const unsigned char* vc = kp + kTileKeys * D / 8;
+    const unsigned char* vp = vc + kTileKeys * D / 2;
+
+    // scores of 64 keys x 8 NT columns
+    float sc[4][NT][4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[mt][n][i] = 0.f;
+      const int ka = mt * 16 + key_a, kb = ka + 8;
+#pragma unroll
+      for (int gr = 0; gr < kG; ++gr) {
+        const uint32_t wa = *reinterpret_cast<const uint32_t*>(kc + ka * (D / 2) + 16 * gr + 4 * t);
+        const uint32_t wb = *reinterpret_cast<const uint32_t*>(kc + kb * (D / 2) + 16 * gr + 4 * t);
+        const uint32_t pa = *reinterpret_cast<const uint32_t*>(kp + ka * (D / 8) + 4 * gr);
+        const uint32_t pb = *reinterpret_cast<const uint32_t*>(kp + kb * (D / 8) + 4 * gr);
+        uint32_t a[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          a[i][0] = codes_bf16(wa >> (8 * i));
+          a[i][1] = codes_bf16(wb >> (8 * i));
+          a[i][2] = codes_bf16(wa >> (8 * i + 4));
+          a[i][3] = codes_bf16(wb >> (8 * i + 4));
+        }
+        const float sa = bf16_lo(pa), sb = bf16_lo(pb);
+        const float za = fmaf(8.f, sa, bf16_hi(pa)), zb = fmaf(8.f, sb, bf16_hi(pb));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int part = 0; part < S::kQParts; ++part) {
+            mma_bf16(c, a[0], qf[gr][part][n][0], qf[gr][part][n][1]);
+            mma_bf16(c, a[1], qf[gr][part][n][2], qf[gr][part][n][3]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float sg = i < 2 ? sa : sb, zg = i < 2 ? za : zb;
+            sc[mt][n][i] = fmaf(sg, c[i], fmaf(zg, qsum[gr][n][i & 1], sc[mt][n][i]));
+          }
+        }
+      }
+    }
+    // scale, mask, running maximum
+    float alpha[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int l = l0 + mt * 16 + key_a + (i < 2 ? 0 : 8);
+          const bool seen = there && l < limit[n][i & 1];
+          const float v = seen ? sc[mt][n][i] * p.scale_log2 : -INFINITY;
+          sc[mt][n][i] = v;
+          top[i & 1] = fmaxf(top[i & 1], v);
+          if constexpr (kLogits) {
+            const int col = col0 + 8 * n + 2 * t + (i & 1);
+            if (col < p.n_cols && key0 + l < key1)
+              p.logits[(((int64_t)b * p.c.n_kv + h) * p.n_cols + col) * p.logit_stride + key0 + l] = v;
+          }
+        }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xFFFFFFFFu, top[j], o));
+        const float m_new = fmaxf(m_run[n][j], top[j]);
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        alpha[n][j] = ex2(m_run[n][j] - m_use);
+        m_run[n][j] = m_new;
+        l_run[n][j] *= alpha[n][j];
+        top[j] = m_use;
+      }
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v = ex2(sc[mt][n][i] - top[i & 1]);
+          sc[mt][n][i] = v;
+          l_run[n][i & 1] += v;
+        }
+#pragma unroll
+      for (int gr = 0; gr < kG; ++gr) {
+        zsum[gr][n][0] *= alpha[n][0];
+        zsum[gr][n][1] *= alpha[n][1];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          acc[gr][i][n][0] *= alpha[n][0];
+          acc[gr][i][n][1] *= alpha[n][1];
+          acc[gr][i][n][2] *= alpha[n][0];
+          acc[gr][i][n][3] *= alpha[n][1];
+        }
+      }
+    }
+    // output: channels x keys
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      const int ka = mt * 16 + key_a, kb = ka + 8;
+#pragma unroll
+      for (int gr = 0; gr < kG; ++gr) {
+        const uint32_t pa = *reinterpret_cast<const uint32_t*>(vp + ka * (D / 8) + 4 * gr);
+        const uint32_t pb = *reinterpret_cast<const uint32_t*>(vp + kb * (D / 8) + 4 * gr);
+        const float sa = bf16_lo(pa), sb = bf16_lo(pb);
+        const float za = fmaf(8.f, sa, bf16_hi(pa)), zb = fmaf(8.f, sb, bf16_hi(pb));
+        uint32_t a[2][4];
+        const unsigned char* word = vc + (mt * 16 + t) * (D / 2) + 16 * gr + 4 * (g >> 1);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(word + (8 * half) * (D / 2));
+          const uint32_t w1 = *reinterpret_cast<const uint32_t*>(word + (8 * half + 4) * (D / 2));
+          const uint32_t byte = 2 * (g & 1);
+          const uint32_t x0 = __byte_perm(w0, w1, 0x4400 + 0x1111 * byte);
+          const uint32_t x1 = __byte_perm(w0, w1, 0x4400 + 0x1111 * (byte + 1));
+          a[0][2 * half] = codes_bf16(x0);
+          a[0][2 * half + 1] = codes_bf16(x0 >> 4);
+          a[1][2 * half] = codes_bf16(x1);
+          a[1][2 * half + 1] = codes_bf16(x1 >> 4);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float ps[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v = sc[mt][n][i], sg = i < 2 ? sa : sb, zg = i < 2 ? za : zb;
+            // a masked key's parameters may be anything
+            ps[i] = v > 0.f || v != v ? v * sg : 0.f;
+            zsum[gr][n][i & 1] += v > 0.f || v != v ? v * zg : 0.f;
+          }
+#pragma unroll
+          for (int part = 0; part < S::kPParts; ++part) {
+            const uint32_t p0 = pack_bf16(ps[0], ps[1]), p1 = pack_bf16(ps[2], ps[3]);
+            const uint32_t b0 = transpose8x8(p0), b1 = transpose8x8(p1);
+            mma_bf16(acc[gr][0][n], a[0], b0, b1);
+            mma_bf16(acc[gr][1][n], a[1], b0, b1);
+            ps[0] -= bf16_lo(p0);
+            ps[1] -= bf16_hi(p0);
+            ps[2] -= bf16_lo(p1);
+            ps[3] -= bf16_hi(p1);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    if (it + kStages < my_tiles) issue(it + kStages, base);
+  }
+  if (failed) {
+    // the copies still in flight must land before this CTA's shared memory goes to another
+    for (int it = failed_at; it < min(failed_at + kStages, my_tiles); ++it)
+      mbar_wait(bar0 + 8 * (it % kStages), (it / kStages) & 1);
+    if (lane == 0 && p.status) atomicExch(p.status, SVA_ERR_TIMEOUT);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) l_run[n][0] = l_run[n][1] = NAN;
+  }
+  // the four warps' states meet in shared memory; every copy issued has been waited for unless a wait
+  // failed, and then the ring is not reused
+  __shared__ float w_m[kDecWarps][S::kCols], w_l[kDecWarps][S::kCols];
+  __shared__ int any_failed;
+  if (threadIdx.x == 0) any_failed = 0;
+  __syncthreads();
+  if (failed) any_failed = 1;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        l_run[n][j] += __shfl_xor_sync(0xFFFFFFFFu, l_run[n][j], o);
+#pragma unroll
+        for (int gr = 0; gr < kG; ++gr) zsum[gr][n][j] += __shfl_xor_sync(0xFFFFFFFFu, zsum[gr][n][j], o);
+      }
+      if (g == 0) {
+        w_m[warp][8 * n + 2 * t + j] = m_run[n][j];
+        w_l[warp][8 * n + 2 * t + j] = l_run[n][j];
+      }
+    }
+  __syncthreads();
+  float* w_o = reinterpret_cast<float*>(smem + 128);  // [warp][column][D]
+  if (!any_failed) {
+#pragma unroll
+    for (int gr = 0; gr < kG; ++gr)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float z = zsum[gr][n][j];
+          *reinterpret_cast<float4*>(w_o + (warp * S::kCols + 8 * n + 2 * t + j) * D + kGroup * gr + 4 * g) =
+              make_float4(acc[gr][0][n][j] + z, acc[gr][0][n][2 + j] + z, acc[gr][1][n][j] + z, acc[gr][1][n][2 + j] + z);
+        }
+  }
+  __syncthreads();
+  const bool last = p.n_chunks == 1;
+  const int64_t problem = ((int64_t)b * p.c.n_kv + h) * p.col_tiles + ct;
+  for (int e = threadIdx.x; e < S::kCols * D; e += blockDim.x) {
+    const int c = e / D, d = e % D, col = col0 + c;
+    if (col >= p.n_cols) break;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) top = fmaxf(top, w_m[w][c]);
+    const float use = top == -INFINITY ? 0.f : top;
+    float l = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) {
+      const float f = ex2(w_m[w][c] - use);
+      l = fmaf(f, w_l[w][c], l);
+      o = any_failed ? NAN : fmaf(f, w_o[(w * S::kCols + c) * D + d], o);
+    }
+    if (last) {
+      const int tok = col / p.groups, head = h * p.groups + col % p.groups;
+      const bool none = top == -INFINITY && l == 0.f;
+      reinterpret_cast<T*>(p.out)[b * p.o_seq + (int64_t)head * p.o_head + (int64_t)tok * p.o_row + d] =
+          from_f32<T>(none ? 0.f : o / l);
+      if (p.lse && d == 0)
+        p.lse[((int64_t)b * p.n_heads + head) * p.n_tokens + tok] = none ? -INFINITY : (use + log2f(l)) / kLog2e;
+    } else {
+      p.part_o[((problem * p.n_chunks + chunk) * S::kCols + c) * D + d] = o;
+    }
+    if (d == 0 && (!last || kLogits)) {
+      float* ml = p.part_ml + ((problem * p.n_chunks + chunk) * S::kCols + c) * 2;
+      ml[0] = top;
+      ml[1] = l;
+    }
+  }
+}
+
+// Joins the chunks of one (sequence, kv head, column): blockIdx.x < n_cols; the blocks behind add the
+// softmax weights of 1024 keys each.
+template <typename T, int D, int COLS>
+__global__ void __launch_bounds__(512) kv4_join_kernel(const Kv4DecParams p) {
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int64_t len = seq_len_of(p, b);
+  const int chunks = max((int)((len + p.chunk_keys - 1) / p.chunk_keys), 1);
+  const int tid = threadIdx.x;
+  const int join_blocks = p.n_chunks > 1 ? p.n_cols : 0;
+  __shared__ float red[16];
+  __shared__ float bc;
+  __shared__ float part[512];
+  auto stats = [&](int col, float* top_out, float* l_out) {  // maximum and sum of a column over its chunks
+    const int64_t problem = ((int64_t)b * p.c.n_kv + h) * p.col_tiles + col / COLS;
+    const float* ml = p.part_ml + (problem * p.n_chunks * COLS + col % COLS) * 2;
+    float top = -INFINITY;
+    for (int c = tid; c < chunks; c += 512) top = fmaxf(top, ml[(int64_t)c * COLS * 2]);
+    top = warp_max(top);
+    if ((tid & 31) == 0) red[tid >> 5] = top;
+    __syncthreads();
+    if (tid < 32) {
+      top = warp_max(tid < 16 ? red[tid] : -INFINITY);
+      if (tid == 0) bc = top;
+    }
+    __syncthreads();
+    top = bc;
+    const float use = top == -INFINITY ? 0.f : top;
+    float l = 0.f;
+    for (int c = tid; c < chunks; c += 512) l = fmaf(ex2(ml[(int64_t)c * COLS * 2] - use), ml[(int64_t)c * COLS * 2 + 1], l);
+    l = warp_sum(l);
+    if ((tid & 31) == 0) red[tid >> 5] = l;
+    __syncthreads();
+    if (tid < 32) {
+      l = warp_sum(tid < 16 ? red[tid] : 0.f);
+      if (tid == 0) bc = l;
+    }
+    __syncthreads();
+    *top_out = top;
+    *l_out = bc;
+    __syncthreads();
+  };
+  if ((int)blockIdx.x < join_blocks) {
+    const int col = blockIdx.x;
+    float top, l;
+    stats(col, &top, &l);
+    const float use = top == -INFINITY ? 0.f : top;
+    const int64_t problem = ((int64_t)b * p.c.n_kv + h) * p.col_tiles + col / COLS;
+    const int64_t first = problem * p.n_chunks * COLS + col % COLS;
+    const int d = tid % D;
+    float o = 0.f;
+#pragma unroll 4
+    for (int c = tid / D; c < chunks; c += 512 / D) {
+      const int64_t at = first + (int64_t)c * COLS;
+      o = fmaf(ex2(p.part_ml[at * 2] - use), p.part_o[at * D + d], o);
+    }
+    part[tid] = o;
+    __syncthreads();
+    if (tid < D) {
+      for (int i = 1; i < 512 / D; ++i) o += part[tid + i * D];
+      const int tok = col / p.groups, head = h * p.groups + col % p.groups;
+      const bool none = top == -INFINITY && l == 0.f;
+      reinterpret_cast<T*>(p.out)[b * p.o_seq + (int64_t)head * p.o_head + (int64_t)tok * p.o_row + tid] =
+          from_f32<T>(none ? 0.f : o / l);
+      if (p.lse && tid == 0)
+        p.lse[((int64_t)b * p.n_heads + head) * p.n_tokens + tok] = none ? -INFINITY : (use + log2f(l)) / kLog2e;
+    }
+    return;
+  }
+  const int64_t l0 = (int64_t)(blockIdx.x - join_blocks) * 1024;
+  if (l0 >= len) return;
+  float sum[2] = {0.f, 0.f};
+  for (int col = 0; col < p.n_cols; ++col) {
+    float top, l;
+    stats(col, &top, &l);
+    if (top == -INFINITY && l == 0.f) continue;
+    const float* row = p.logits + (((int64_t)b * p.c.n_kv + h) * p.n_cols + col) * p.logit_stride;
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int64_t key = l0 + j * 512 + tid;
+      if (key < len) sum[j] = fmaf(ex2(row[key] - top), inv, sum[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int64_t key = l0 + j * 512 + tid;
+    if (key < len) p.weights[b * p.w_seq + h * p.w_head + key] += sum[j];
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------
+static int check_cache(const sva_kv4_cache* c, int n_seqs, Kv4* out) {
+  if (!c) return set_error(SVA_ERR_SHAPE, "the cache is null");
+  if (c->head_dim != 64 && c->head_dim != 128) return set_error(SVA_ERR_SHAPE, "a 4-bit cache takes head_dim 64 or 128");
+  if (c->n_kv_heads <= 0 || c->n_pages <= 0 || c->page_rows <= 0 || c->page_rows % kTileKeys || c->page_rows > (1ll << 31))
+    return set_error(SVA_ERR_SHAPE, "the cache needs pages of a multiple of 64 rows");
+  if (!c->k_codes || !c->k_params || !c->v_codes || !c->v_params) return set_error(SVA_ERR_SHAPE, "a cache pointer is null");
+  const void* ptrs[4] = {c->k_codes, c->k_params, c->v_codes, c->v_params};
+  for (const void* q : ptrs)
+    if (reinterpret_cast<uintptr_t>(q) % 16) return set_error(SVA_ERR_ALIGN, "the cache must be 16-byte aligned");
+  if (n_seqs <= 0 || n_seqs > 65535) return set_error(SVA_ERR_SHAPE, "n_seqs must be in 1..65535");
+  int shift = 0;
+  if (c->page_table) {
+    while ((1ll << shift) < c->page_rows) ++shift;
+    if ((1ll << shift) != c->page_rows) return set_error(SVA_ERR_SHAPE, "with a page table page_rows must be a power of two");
+    if (c->page_table_cols <= 0 || c->page_table_stride < 0) return set_error(SVA_ERR_SHAPE, "bad page table sizes");
+  } else if (c->n_pages < n_seqs) {
+    return set_error(SVA_ERR_SHAPE, "the cache has fewer pages than there are sequences, and no page table");
+  }
+  *out = Kv4{c->n_pages, c->page_rows, c->n_kv_heads, shift, static_cast<uint8_t*>(c->k_codes),
+             static_cast<uint32_t*>(c->k_params), static_cast<uint8_t*>(c->v_codes), static_cast<uint32_t*>(c->v_params),
+             c->page_table, c->page_table_stride, c->page_table_cols};
+  return SVA_OK;
+}
+
+static int launched() {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? SVA_OK : set_error(SVA_ERR_CUDA, cudaGetErrorString(e));
+}
+
+template <typename T>
+static int launch_write(const Kv4WriteParams& p, int D, bool packed, cudaStream_t st) {
+  const int64_t rows = 4 * (256 / (D / 8));
+  const int64_t blocks = (p.n_tokens + rows - 1) / rows;
+  const int64_t ys = (int64_t)p.c.n_kv * (packed ? 1 : p.n_seqs);
+  if (blocks > 0x7FFFFFFFll || ys > 65535) return set_error(SVA_ERR_SHAPE, "too many rows, or sequences times kv heads");
+  const dim3 grid((unsigned)blocks, (unsigned)ys, 2);
+  if (D == 64)
+    kv4_write_kernel<T, 64><<<grid, 256, 0, st>>>(p);
+  else
+    kv4_write_kernel<T, 128><<<grid, 256, 0, st>>>(p);
+  return launched();
+}
+
+template <typename T>
+static int launch_read(const Kv4ReadParams& p, int D, int n_seqs, cudaStream_t st) {
+  const int64_t rows = 4 * (256 / (D / 8));
+  const int64_t blocks = (p.n_tokens + rows - 1) / rows;
+  const int64_t ys = (int64_t)p.c.n_kv * n_seqs;
+  if (blocks > 0x7FFFFFFFll || ys > 65535) return set_error(SVA_ERR_SHAPE, "too many rows, or sequences times kv heads");
+  const dim3 grid((unsigned)blocks, (unsigned)ys, 2);
+  if (D == 64)
+    kv4_read_kernel<T, 64><<<grid, 256, 0, st>>>(p);
+  else
+    kv4_read_kernel<T, 128><<<grid, 256, 0, st>>>(p);
+  return launched();
+}
+
+struct DecPlan {
+  int cols, col_tiles, n_cols, chunks;
+  int64_t chunk_keys, logit_stride;
+  size_t ml, o, logits, total;  // byte offsets into the workspace, and its size
+};
+
+static int plan_decode(const sva_kv4_cache* c, const sva_kv4_decode_args* a, Kv4* cache, DecPlan* plan) {
+  if (!a) return set_error(SVA_ERR_SHAPE, "the arguments are null");
+  int rc = check_cache(c, a->n_seqs, cache);
+  if (rc != SVA_OK) return rc;
+  if (a->n_heads <= 0 || a->n_heads % c->n_kv_heads) return set_error(SVA_ERR_SHAPE, "n_heads must be a multiple of the cache's kv heads");
+  if (a->n_tokens <= 0) return set_error(SVA_ERR_SHAPE, "n_tokens must be positive");
+  const int64_t capacity = c->page_table ? c->page_table_cols * c->page_rows : c->page_rows;
+  if (a->max_len < 0 || a->max_len > capacity || a->max_len >= (1ll << 31))
+    return set_error(SVA_ERR_SHAPE, "max_len must be within the cache's capacity and below 2^31");
+  if (a->dtype < 0 || a->dtype > 2) return set_error(SVA_ERR_DTYPE, "dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
+  const int64_t n_cols = (int64_t)(a->n_heads / c->n_kv_heads) * a->n_tokens;
+  // 16 columns a CTA where there are more than 8 (16-bit types): one pass over the cache instead of two
+  plan->cols = (n_cols > 8 && a->dtype != SVA_DTYPE_F32) ? 16 : 8;
+  const int64_t tiles = (n_cols + plan->cols - 1) / plan->cols;
+  if (n_cols > (1 << 20) || tiles * c->n_kv_heads > 65535) return set_error(SVA_ERR_SHAPE, "too many tokens times heads");
+  plan->n_cols = (int)n_cols;
+  plan->col_tiles = (int)tiles;
+  const int64_t problems = (int64_t)a->n_seqs * c->n_kv_heads * plan->col_tiles;
+  const int64_t slots = 148 * 3;  // CTAs that fit the GPU at once
+  const int64_t tiles_k = std::max<int64_t>(1, (a->max_len + kTileKeys - 1) / kTileKeys);
+  int64_t chunks = std::max<int64_t>(1, slots / problems);
+  // at least 4 tiles a CTA (one a warp); at most 64 where lengths differ, so that long sequences spread
+  int64_t per = (tiles_k + chunks - 1) / chunks;
+  per = std::max<int64_t>(per, kDecWarps);
+  if (a->seq_lens) per = std::min<int64_t>(per, 64);
+  per = (per + kDecWarps - 1) / kDecWarps * kDecWarps;
+  chunks = (tiles_k + per - 1) / per;
+  plan->chunks = (int)chunks;
+  plan->chunk_keys = per * kTileKeys;
+  plan->logit_stride = a->max_len;
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  const bool parts = chunks > 1;
+  plan->ml = 0;
+  size_t at = (parts || a->weights) ? up((size_t)problems * chunks * plan->cols * 2 * 4) : 0;
+  plan->o = at;
+  if (parts) at += up((size_t)problems * chunks * plan->cols * c->head_dim * 4);
+  plan->logits = at;
+  if (a->weights) at += up((size_t)a->n_seqs * c->n_kv_heads * n_cols * a->max_len * 4);
+  plan->total = at;
+  return SVA_OK;
+}
+
+template <typename T, int D, int NT>
+static int launch_decode(Kv4DecParams& p, int n_seqs, cudaStream_t st) {
+  using S = DecShape<T, D, NT>;
+  const dim3 grid(p.n_chunks, p.c.n_kv * p.col_tiles, n_seqs);
+  auto* kern = p.weights ? kv4_decode_kernel<T, D, NT, true> : kv4_decode_kernel<T, D, NT, false>;
+  int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), S::kSmem);
+  if (rc != SVA_OK) return rc;
+  kern<<<grid, kDecWarps * 32, S::kSmem, st>>>(p);
+  rc = launched();
+  if (rc != SVA_OK) return rc;
+  const int64_t wblocks = p.weights ? (p.max_len + 1023) / 1024 : 0;
+  const int64_t jblocks = (p.n_chunks > 1 ? p.n_cols : 0) + wblocks;
+  if (jblocks == 0) return SVA_OK;
+  kv4_join_kernel<T, D, 8 * NT><<<dim3((unsigned)jblocks, p.c.n_kv, n_seqs), 512, 0, st>>>(p);
+  return launched();
+}
+
+template <typename T>
+static int decode_dims(Kv4DecParams& p, int D, int cols, int n_seqs, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (cols == 16) return D == 64 ? launch_decode<T, 64, 2>(p, n_seqs, st) : launch_decode<T, 128, 2>(p, n_seqs, st);
+  }
+  return D == 64 ? launch_decode<T, 64, 1>(p, n_seqs, st) : launch_decode<T, 128, 1>(p, n_seqs, st);
+}
+
+}  // namespace sva
+
+using namespace sva;
+
+extern "C" int sva_kv4_write(const sva_kv4_cache* cache, const void* keys, int64_t k_seq_stride, int64_t k_head_stride,
+                             int64_t k_row_stride, const void* values, int64_t v_seq_stride, int64_t v_head_stride,
+                             int64_t v_row_stride, int32_t dtype, int32_t n_seqs, int64_t n_tokens,
+                             const int64_t* start, const int64_t* cu_seqlens, void* stream) {
+  Kv4WriteParams p{};
+  int rc = check_cache(cache, n_seqs, &p.c);
+  if (rc != SVA_OK) return rc;
+  if (n_tokens < 0) return set_error(SVA_ERR_SHAPE, "n_tokens must not be negative");
+  if (dtype < 0 || dtype > 2) return set_error(SVA_ERR_DTYPE, "dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
+  if (n_tokens == 0) return SVA_OK;
+  if (!keys || !values || !start) return set_error(SVA_ERR_SHAPE, "a required pointer is null");
+  const int64_t strides[2][3] = {{k_seq_stride, k_head_stride, k_row_stride}, {v_seq_stride, v_head_stride, v_row_stride}};
+  const void* ptr[2] = {keys, values};
+  const int size = dtype == SVA_DTYPE_F32 ? 4 : 2;
+  for (int i = 0; i < 2; ++i) {
+    p.x[i] = ptr[i];
+    p.seq_stride[i] = cu_seqlens ? 0 : strides[i][0];
+    p.head_stride[i] = strides[i][1];
+    p.row_stride[i] = strides[i][2];
+    p.vec[i] = reinterpret_cast<uintptr_t>(ptr[i]) % 16 == 0 && p.seq_stride[i] * size % 16 == 0 &&
+               p.head_stride[i] * size % 16 == 0 && p.row_stride[i] * size % 16 == 0;
+  }
+  p.n_seqs = n_seqs;
+  p.n_tokens = n_tokens;
+  p.start = start;
+  p.cu = cu_seqlens;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool packed = cu_seqlens != nullptr;
+  switch (dtype) {
+    case SVA_DTYPE_F32: return launch_write<float>(p, cache->head_dim, packed, st);
+    case SVA_DTYPE_BF16: return launch_write<__nv_bfloat16>(p, cache->head_dim, packed, st);
+    default: return launch_write<__half>(p, cache->head_dim, packed, st);
+  }
+}
+
+extern "C" int sva_kv4_read(const sva_kv4_cache* cache, void* keys_out, void* values_out, int32_t dtype, int32_t n_seqs,
+                            int64_t n_tokens, const int64_t* start, void* stream) {
+  Kv4ReadParams p{};
+  int rc = check_cache(cache, n_seqs, &p.c);
+  if (rc != SVA_OK) return rc;
+  if (n_tokens < 0) return set_error(SVA_ERR_SHAPE, "n_tokens must not be negative");
+  if (dtype < 0 || dtype > 2) return set_error(SVA_ERR_DTYPE, "dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
+  if (n_tokens == 0) return SVA_OK;
+  if (!keys_out || !values_out || !start) return set_error(SVA_ERR_SHAPE, "a required pointer is null");
+  if (reinterpret_cast<uintptr_t>(keys_out) % 16 || reinterpret_cast<uintptr_t>(values_out) % 16)
+    return set_error(SVA_ERR_ALIGN, "the outputs must be 16-byte aligned");
+  p.out[0] = keys_out;
+  p.out[1] = values_out;
+  p.n_tokens = n_tokens;
+  p.start = start;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case SVA_DTYPE_F32: return launch_read<float>(p, cache->head_dim, n_seqs, st);
+    case SVA_DTYPE_BF16: return launch_read<__nv_bfloat16>(p, cache->head_dim, n_seqs, st);
+    default: return launch_read<__half>(p, cache->head_dim, n_seqs, st);
+  }
+}
+
+extern "C" size_t sva_kv4_decode_workspace_size(const sva_kv4_cache* cache, const sva_kv4_decode_args* args) {
+  Kv4 c;
+  DecPlan plan;
+  return plan_decode(cache, args, &c, &plan) == SVA_OK ? plan.total : 0;
+}
+
+extern "C" int sva_kv4_decode(const sva_kv4_cache* cache, const sva_kv4_decode_args* a, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  Kv4DecParams p{};
+  DecPlan plan;
+  int rc = plan_decode(cache, a, &p.c, &plan);
+  if (rc != SVA_OK) return rc;
+  if (!a->query || !a->out) return set_error(SVA_ERR_SHAPE, "a required pointer is null");
+  if (plan.total > 0 && (!workspace || workspace_bytes < plan.total)) return set_error(SVA_ERR_WORKSPACE, "workspace too small");
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return set_error(SVA_ERR_ALIGN, "the workspace must be 16-byte aligned");
+  p.q = a->query;
+  p.q_seq = a->q_seq_stride, p.q_head = a->q_head_stride, p.q_row = a->q_row_stride;
+  p.out = a->out;
+  p.o_seq = a->out_seq_stride, p.o_head = a->out_head_stride, p.o_row = a->out_row_stride;
+  p.seq_lens = a->seq_lens;
+  p.max_len = a->max_len;
+  p.scale = a->softmax_scale;
+  p.scale_log2 = a->softmax_scale * kLog2e;
+  p.n_heads = a->n_heads, p.n_tokens = a->n_tokens, p.groups = a->n_heads / cache->n_kv_heads;
+  p.n_cols = plan.n_cols, p.col_tiles = plan.col_tiles, p.n_chunks = plan.chunks, p.chunk_keys = plan.chunk_keys;
+  p.lse = a->lse;
+  p.weights = a->weights;
+  p.w_seq = a->weights_seq_stride, p.w_head = a->weights_head_stride;
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  p.part_ml = reinterpret_cast<float*>(ws + plan.ml);
+  p.part_o = reinterpret_cast<float*>(ws + plan.o);
+  p.logits = reinterpret_cast<float*>(ws + plan.logits);
+  p.logit_stride = plan.logit_stride;
+  p.status = a->status;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (a->dtype) {
+    case SVA_DTYPE_F32: return decode_dims<float>(p, cache->head_dim, plan.cols, a->n_seqs, st);
+    case SVA_DTYPE_BF16: return decode_dims<__nv_bfloat16>(p, cache->head_dim, plan.cols, a->n_seqs, st);
+    default: return decode_dims<__half>(p, cache->head_dim, plan.cols, a->n_seqs, st);
+  }
+}

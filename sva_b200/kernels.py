@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from typing import NamedTuple, Sequence
 
 import torch
 
@@ -574,3 +575,306 @@ def top_unique(candidate_idx: torch.Tensor, candidate_scores: torch.Tensor, cand
                                     ctypes.byref(refill_out), _stream(dev))
     _lib.check(rc)
     return sel_idx, sel_scores.to(candidate_scores.dtype), sel_valid.bool(), int(refill_out.value)
+
+
+# ------------------------------------------------------------------------------------------
+# attention over every key: whole prompts, a 4-bit cache, eviction
+# ------------------------------------------------------------------------------------------
+
+
+def _same_device(dev: torch.device, **tensors: torch.Tensor | None) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            if not t.is_cuda:
+                _cuda(t, name)
+            raise ValueError(f"{name} is on {t.device}, the call's other tensors on {dev}")
+
+
+def _call(dev: torch.device, fn, *args) -> None:
+    """fn(*args, stream) with ``dev`` as the current device, on its current stream."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc)
+
+
+def _scratch(dev: torch.device, nbytes: int) -> torch.Tensor | None:
+    """Workspace of one call.  It comes from torch's allocator at every call, so that calls on two
+    streams, and graphs captured apart, never share one."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
+
+
+def _int64(t: torch.Tensor, name: str, n: int) -> int:
+    if t.dtype != torch.int64 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int64 tensor of {n} entries")
+    return t.data_ptr()
+
+
+def _page_table(t: torch.Tensor | None, n_seqs: int) -> tuple:
+    """(pointer, row stride, columns) of a page table, or of none."""
+    if t is None:
+        return None, 0, 0
+    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != n_seqs or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"page_table must be an int32 [{n_seqs}, max_pages] tensor with contiguous rows")
+    return t.data_ptr(), t.stride(0), t.shape[1]
+
+
+def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, cu_seqlens: torch.Tensor, *,
+                     cu_seqlens_k: torch.Tensor | None = None, causal: bool = True, softmax_scale: float | None = None,
+                     out: torch.Tensor | None = None, want_lse: bool = False, status: torch.Tensor | None = None):
+    """Attention over whole prompts packed without padding (sva_prompt_attention).
+
+    q [N, H, D]; keys / values [Nk, Hkv, D] (any strides with contiguous rows; H a multiple of Hkv, D <= 256);
+    ``cu_seqlens`` [B + 1] int64 on the device: sequence b owns query rows cu_seqlens[b] ..
+    cu_seqlens[b + 1] - 1, and key rows likewise by ``cu_seqlens_k`` (None: the same).  With Lq query and Lk key
+    rows, query i sees keys j <= i + Lk - Lq, so new tokens may follow a cached beginning; ``causal``
+    False: all Lk.  A query that sees no key gets zeros; rows behind the last sequence are left as they
+    were.  Returns out [N, H, D] (and the log-sum-exp [H, N] fp32 with ``want_lse``).  bf16 and fp16
+    rows of D <= 128 channels, a multiple of 8, run on the tensor cores when every stride is a multiple of 16
+    bytes; other calls on the CUDA cores in fp32.  ``status`` (int32 device scalar) receives a timeout flag.
+    """
+    _cuda(q, "q")
+    dev = q.device
+    _same_device(dev, keys=keys, values=values, cu_seqlens=cu_seqlens, cu_seqlens_k=cu_seqlens_k, out=out, status=status)
+    if q.dim() != 3 or keys.dim() != 3 or values.shape != keys.shape or keys.shape[2] != q.shape[2]:
+        raise ValueError("prompt_attention takes q [N, H, D] and keys / values [Nk, Hkv, D]")
+    if keys.dtype != q.dtype or values.dtype != q.dtype:
+        raise TypeError("q, keys and values must share a dtype")
+    n, n_heads, head_dim = q.shape
+    if head_dim > 1 and (q.stride(2) != 1 or keys.stride(2) != 1 or values.stride(2) != 1):
+        raise ValueError("q, keys and values must have contiguous rows")
+    n_seqs = cu_seqlens.shape[0] - 1 if cu_seqlens.dim() == 1 else -1
+    if n_seqs < 0:
+        raise ValueError("cu_seqlens must be a [B + 1] tensor")
+    if cu_seqlens_k is None and keys.shape[0] != n:
+        raise ValueError("cu_seqlens_k is needed where queries and keys differ in number")
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape or out.dtype != q.dtype or (head_dim > 1 and out.stride(2) != 1):
+        raise ValueError("out must have q's shape and dtype, with contiguous rows")
+    lse = torch.full((n_heads, n), float("-inf"), dtype=torch.float32, device=dev) if want_lse else None
+    a = _lib.PromptArgs(n_seqs, n_heads, keys.shape[1], head_dim, dtype_code(q.dtype), int(causal),
+                        head_dim ** -0.5 if softmax_scale is None else softmax_scale, n, keys.shape[0],
+                        q.data_ptr(), q.stride(0), q.stride(1), keys.data_ptr(), keys.stride(0), keys.stride(1),
+                        values.data_ptr(), values.stride(0), values.stride(1),
+                        _int64(cu_seqlens, "cu_seqlens", n_seqs + 1),
+                        None if cu_seqlens_k is None else _int64(cu_seqlens_k, "cu_seqlens_k", n_seqs + 1),
+                        out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse), _ptr(status))
+    lib = _lib.load()
+    ref = ctypes.byref(a)
+    nbytes = lib.sva_prompt_attention_workspace_size(ref)
+    ws = _scratch(dev, nbytes)
+    _call(dev, lib.sva_prompt_attention, ref, _ptr(ws), nbytes)
+    return (out, lse) if want_lse else out
+
+
+class Kv4Cache(NamedTuple):
+    """A key/value cache in 4 bits (see include/sva_b200.h for the format): codes [pages, Hkv, rows, D / 2]
+    uint8 and parameters [pages, Hkv, rows, D / 32, 2] bf16 (scale, minimum) of the keys and of the values.
+    A page is a sequence when calls get no page table."""
+
+    k_codes: torch.Tensor
+    k_params: torch.Tensor
+    v_codes: torch.Tensor
+    v_params: torch.Tensor
+
+
+def kv4_empty(pages: int, n_kv_heads: int, rows: int, head_dim: int, device="cuda") -> Kv4Cache:
+    """An uninitialised 4-bit cache of ``pages`` pages (or sequences) of ``rows`` rows (a multiple of 64)."""
+    if head_dim not in (64, 128):
+        raise ValueError("a 4-bit cache takes head_dim 64 or 128")
+    if rows <= 0 or rows % 64:
+        raise ValueError("rows must be a positive multiple of 64")
+    return Kv4Cache(*(torch.empty(pages, n_kv_heads, rows, *tail, dtype=dtype, device=device)
+                      for tail, dtype in (((head_dim // 2,), torch.uint8), ((head_dim // 32, 2), torch.bfloat16)) * 2))
+
+
+def _kv4_args(cache: Kv4Cache, n_seqs: int, page_table: torch.Tensor | None) -> _lib.Kv4CacheArgs:
+    kc, kp, vc, vp = cache
+    dev = _cuda(kc, "k_codes").device
+    _same_device(dev, k_params=kp, v_codes=vc, v_params=vp, page_table=page_table)
+    if kc.dim() != 4 or kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or vc.shape != kc.shape:
+        raise ValueError("codes must be uint8 [pages, Hkv, rows, D / 2]")
+    pages, n_kv, rows, half = kc.shape
+    tail = (pages, n_kv, rows, half // 16, 2)
+    if kp.dtype != torch.bfloat16 or vp.dtype != torch.bfloat16 or kp.shape != tail or vp.shape != tail:
+        raise ValueError("parameters must be bfloat16 [pages, Hkv, rows, D / 32, 2]")
+    if not (kc.is_contiguous() and kp.is_contiguous() and vc.is_contiguous() and vp.is_contiguous()):
+        raise ValueError("the cache's tensors must be contiguous")
+    return _lib.Kv4CacheArgs(pages, rows, n_kv, half * 2, kc.data_ptr(), kp.data_ptr(), vc.data_ptr(), vp.data_ptr(),
+                             *_page_table(page_table, n_seqs))
+
+
+def kv4_write(keys: torch.Tensor, values: torch.Tensor, cache: Kv4Cache, start: torch.Tensor, *,
+              page_table: torch.Tensor | None = None, cu_seqlens: torch.Tensor | None = None) -> None:
+    """Quantises rows into the 4-bit cache (sva_kv4_write).
+
+    keys / values [B, Hkv, T, D]: token t of sequence b goes to position start[b] + t; or packed
+    [N, Hkv, D] with ``cu_seqlens`` [B + 1]: row n of sequence b goes to start[b] + n - cu_seqlens[b], and rows of no
+    sequence are skipped.  ``start`` [B] int64 on the device, so that a captured graph may append at a moving
+    position.  Positions outside the cache are skipped.
+    """
+    _cuda(keys, "keys")
+    packed = cu_seqlens is not None
+    if keys.dim() != (3 if packed else 4) or values.shape != keys.shape:
+        raise ValueError("kv4_write takes keys and values [B, Hkv, T, D], or [N, Hkv, D] with cu_seqlens")
+    if values.dtype != keys.dtype:
+        raise TypeError("keys and values must share a dtype")
+    dev = keys.device
+    _same_device(dev, values=values, start=start, cu_seqlens=cu_seqlens, k_codes=cache.k_codes)
+    if keys.stride(-1) != 1 or values.stride(-1) != 1:
+        raise ValueError("keys and values must have contiguous rows")
+    n_seqs = start.shape[0] if start.dim() == 1 else -1
+    c = _kv4_args(cache, n_seqs, page_table)
+    if keys.shape[1] != c.n_kv_heads or keys.shape[-1] != c.head_dim or (not packed and keys.shape[0] != n_seqs):
+        raise ValueError("keys do not match the cache's heads, head_dim or start's sequences")
+    order = (lambda t: (0, t.stride(1), t.stride(0))) if packed else (lambda t: t.stride()[:3])
+    if n_seqs == 0 or keys.numel() == 0:
+        return
+    _call(dev, _lib.load().sva_kv4_write, ctypes.byref(c), keys.data_ptr(), *order(keys), values.data_ptr(),
+          *order(values), dtype_code(keys.dtype), n_seqs, keys.shape[0] if packed else keys.shape[2],
+          _int64(start, "start", n_seqs), None if cu_seqlens is None else _int64(cu_seqlens, "cu_seqlens", n_seqs + 1))
+
+
+def kv4_read(cache: Kv4Cache, start: torch.Tensor, count: int, *, dtype: torch.dtype = torch.bfloat16,
+             page_table: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Positions start[b] .. start[b] + count - 1 of every sequence back in ``dtype`` (sva_kv4_read): keys and
+    values [B, Hkv, count, D]; zeros where a position lies outside the cache.  ``start`` [B] int64, device."""
+    dev = _cuda(cache.k_codes, "k_codes").device
+    _same_device(dev, start=start)
+    n_seqs = start.shape[0] if start.dim() == 1 else -1
+    c = _kv4_args(cache, n_seqs, page_table)
+    if count < 0:
+        raise ValueError("count must not be negative")
+    code = dtype_code(dtype)
+    out = torch.empty(2, n_seqs, c.n_kv_heads, count, c.head_dim, dtype=dtype, device=dev)
+    if out.numel() > 0:
+        _call(dev, _lib.load().sva_kv4_read, ctypes.byref(c), out[0].data_ptr(), out[1].data_ptr(), code, n_seqs, count,
+              _int64(start, "start", n_seqs))
+    return out[0], out[1]
+
+
+def kv4_decode(q: torch.Tensor, cache: Kv4Cache, *, seq_lens: torch.Tensor | None = None,
+               page_table: torch.Tensor | None = None, max_len: int | None = None, softmax_scale: float | None = None,
+               out: torch.Tensor | None = None, weights: torch.Tensor | None = None, want_lse: bool = False,
+               status: torch.Tensor | None = None):
+    """Attention of each sequence's newest T tokens over its whole 4-bit cache (sva_kv4_decode).
+
+    q [B, H, T, D] (contiguous rows).  Sequence b holds ``seq_lens[b]`` keys, the T new ones among them ([B] int64
+    on the device; None: ``max_len``), and its token t sees the first seq_lens[b] - T + t + 1.  ``max_len`` (host)
+    bounds the lengths (default: the cache's capacity).  ``weights`` [B, Hkv, >= max_len] fp32: every key's softmax
+    weight, summed over the tokens and the heads that share its kv head, is added in place (``cache_evict``
+    goes by these sums).  Returns out [B, H, T, D] (and the log-sum-exp [B, H, T] fp32 with ``want_lse``).
+    A token that sees no key gets zeros.
+    """
+    _cuda(q, "q")
+    dev = q.device
+    if q.dim() != 4:
+        raise ValueError("kv4_decode takes q [B, H, T, D]")
+    n_seqs, n_heads, n_tokens, head_dim = q.shape
+    _same_device(dev, k_codes=cache.k_codes, seq_lens=seq_lens, out=out, weights=weights, status=status)
+    c = _kv4_args(cache, n_seqs, page_table)
+    if head_dim != c.head_dim or q.stride(3) != 1:
+        raise ValueError("q must have contiguous rows of the cache's head_dim")
+    if max_len is None:
+        max_len = c.page_rows * (c.page_table_cols if page_table is not None else 1)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1:
+        raise ValueError("out must have q's shape and dtype, with contiguous rows")
+    if weights is not None and (weights.dtype != torch.float32 or weights.dim() != 3 or weights.stride(2) != 1
+                                or weights.shape[:2] != (n_seqs, c.n_kv_heads) or weights.shape[2] < max_len):
+        raise ValueError("weights must be float32 [B, Hkv, >= max_len] with contiguous rows")
+    lse = torch.empty(n_seqs, n_heads, n_tokens, dtype=torch.float32, device=dev) if want_lse else None
+    a = _lib.Kv4DecodeArgs(n_seqs, n_heads, n_tokens, dtype_code(q.dtype), max_len,
+                           head_dim ** -0.5 if softmax_scale is None else softmax_scale, q.data_ptr(), *q.stride()[:3],
+                           None if seq_lens is None else _int64(seq_lens, "seq_lens", n_seqs), out.data_ptr(),
+                           *out.stride()[:3], _ptr(lse), _ptr(weights),
+                           *((0, 0) if weights is None else weights.stride()[:2]), _ptr(status))
+    if q.numel() > 0:
+        lib = _lib.load()
+        refs = ctypes.byref(c), ctypes.byref(a)
+        nbytes = lib.sva_kv4_decode_workspace_size(*refs)
+        ws = _scratch(dev, nbytes)
+        _call(dev, lib.sva_kv4_decode, *refs, _ptr(ws), nbytes)
+    return (out, lse) if want_lse else out
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """First byte of a tensor and the byte behind its last."""
+    first = t.data_ptr()
+    return first, first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
+def cache_evict(rows: Sequence[torch.Tensor], weights: torch.Tensor, seq_lens: torch.Tensor, keep: int, *,
+                recent: int = 0, page_table: torch.Tensor | None = None, out: Sequence[torch.Tensor] | None = None,
+                out_weights: torch.Tensor | None = None, out_page_table: torch.Tensor | None = None):
+    """Cuts each sequence's cache down to ``keep`` rows a kv head by accumulated weight (sva_cache_evict).
+
+    ``rows``: up to 8 tensors [pages, Hkv, page_rows, ...] (keys, values, or the members of a ``Kv4Cache``), rows
+    contiguous; without a page table a page is a sequence.  ``weights`` [B, Hkv, >= longest] fp32 (as ``kv4_decode``
+    sums them) and ``seq_lens`` [B] int64.  A sequence of at most ``keep`` rows keeps all of them; else the last
+    ``recent`` rows stay and, of the others, those with the largest weights (ties: the first; NaN counts as
+    the largest).  Rows that stay move together in their order, with their weights; weights behind them
+    become 0.  In place, unless ``out`` (and then ``out_weights``, ``out_page_table``) name another cache; in place no
+    page may belong to two sequences.  Returns (kept [B, Hkv, keep] int32: the old positions, ascending,
+    -1 padded; lengths [B] int64).  Append new rows at the returned lengths, and keep the model's own position
+    count for rotary embeddings: rows are not re-rotated.
+    """
+    _cuda(weights, "weights")
+    dev = weights.device
+    in_place = out is None
+    if in_place and (out_weights is not None or out_page_table is not None):
+        raise ValueError("out_weights and out_page_table go with out")
+    if not in_place and out_weights is None:
+        raise ValueError("out needs out_weights")
+    src = list(rows)
+    dst = src if in_place else list(out)
+    if not 1 <= len(src) <= _lib.EVICT_MAX_ARRAYS or len(dst) != len(src):
+        raise ValueError("cache_evict takes 1 to 8 row tensors, and as many outputs")
+    dst_weights = weights if in_place else out_weights
+    dst_table = page_table if in_place else out_page_table
+    n_seqs = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
+    n_kv = src[0].shape[1] if src[0].dim() >= 3 else -1
+    _same_device(dev, seq_lens=seq_lens, page_table=page_table, out_weights=dst_weights, out_page_table=dst_table)
+    for name, w in (("weights", weights), ("out_weights", dst_weights)):
+        if w.dtype != torch.float32 or w.dim() != 3 or w.shape[:2] != (n_seqs, n_kv) or w.stride(2) != 1:
+            raise ValueError(f"{name} must be float32 [B, Hkv, width] with contiguous rows")
+    arrays = (_lib.EvictArray * len(src))()
+    for i, (s, d) in enumerate(zip(src, dst)):
+        _same_device(dev, rows=s, out=d)
+        for t, like in ((s, src[0]), (d, dst[0])):
+            if t.dim() < 3 or t.shape[:3] != like.shape[:3] or t.shape[1] != n_kv or not t[0, 0].is_contiguous():
+                raise ValueError("rows must be [pages, Hkv, page_rows, ...] tensors of one shape with contiguous rows")
+        if s.dtype != d.dtype or s.shape[3:] != d.shape[3:]:
+            raise ValueError("out must have rows of the same shape and dtype")
+        if not in_place and (any(_overlap(d, t) for t in src) or any(_overlap(d, t) for t in dst[:i])):
+            raise ValueError("out must not overlap rows or itself")
+        size = s.element_size()
+        arrays[i] = (s.data_ptr(), d.data_ptr(), math.prod(s.shape[3:]) * size, s.stride(0) * size, s.stride(1) * size,
+                     d.stride(0) * size, d.stride(1) * size)
+    if not in_place and _overlap(weights, dst_weights):
+        raise ValueError("out_weights must not overlap weights")
+    kept = torch.empty(n_seqs, n_kv, max(keep, 0), dtype=torch.int32, device=dev)
+    lens = torch.empty(n_seqs, dtype=torch.int64, device=dev)
+    rows_of = (lambda t, table: t.shape[2] * (table.shape[1] if table is not None else 1))
+    a = _lib.EvictArgs(n_seqs, n_kv, len(src), int(in_place), min(weights.shape[2], rows_of(src[0], page_table)), keep, recent,
+                       _int64(seq_lens, "seq_lens", n_seqs), weights.data_ptr(), weights.stride(0), weights.stride(1),
+                       dst_weights.data_ptr(), dst_weights.stride(0), dst_weights.stride(1), dst_weights.shape[2],
+                       src[0].shape[0], src[0].shape[2], dst[0].shape[0], dst[0].shape[2],
+                       *_page_table(page_table, n_seqs), *_page_table(dst_table, n_seqs), kept.data_ptr(),
+                       lens.data_ptr())
+    if n_seqs > 0:
+        lib = _lib.load()
+        ref = ctypes.byref(a)
+        nbytes = lib.sva_cache_evict_workspace_size(ref)
+        ws = _scratch(dev, nbytes)
+        _call(dev, lib.sva_cache_evict, ref, arrays, _ptr(ws), nbytes)
+    return kept, lens
