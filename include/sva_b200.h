@@ -473,7 +473,7 @@ int sva_adapter_forward(const void* hidden, int64_t hidden_row_stride, const voi
  * n_kv_heads).  Strides in elements; rows (head_dim elements) are contiguous.
  *   out  [n_rows][n_heads][head_dim] by strides; rows outside every sequence are left as they were
  *   lse  (may be NULL) [n_heads][n_rows] fp32: natural logarithm of the sum of exp(scale q.k)
- * Boundaries are clamped to the tensors' rows.  head_dim <= 256.  `status` (device int32, may be
+ * Boundaries must not decrease; they are clamped to the tensors' rows.  head_dim <= 256.  `status` (device int32, may be
  * NULL) is set to SVA_ERR_TIMEOUT if a bounded wait gave up; the rows concerned become NaN.
  * ------------------------------------------------------------------------------------- */
 typedef struct sva_prompt_args {

