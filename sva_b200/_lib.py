@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -346,6 +347,13 @@ class EvictArgs(ctypes.Structure):
     ]
 
 
+def packer(cls: type[ctypes.Structure]) -> struct.Struct:
+    """The C layout of ``cls`` as a struct.Struct: packing its fields' values into bytes, which a pointer
+    argument takes as they are, is several times cheaper than filling a ctypes structure."""
+    kind = {c_i32: "i", c_i64: "q", c_f32: "f", c_vp: "P"}
+    return struct.Struct("@" + "".join(kind[c] for _, c in cls._fields_) + "0q")
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -411,17 +419,17 @@ def load() -> ctypes.CDLL:
                                 ctypes.POINTER(ctypes.c_int32), c_vp], ctypes.c_int),
             "sva_adapter_forward": ([c_vp, c_i64, c_vp, c_i64, c_i32, c_vp, c_vp, c_vp, c_vp, c_f32, c_i32, c_i32,
                                      c_i32, c_i32, c_vp, c_i64, c_vp], ctypes.c_int),
-            "sva_prompt_attention_workspace_size": ([ctypes.POINTER(PromptArgs)], c_sz),
-            "sva_prompt_attention": ([ctypes.POINTER(PromptArgs), c_vp, c_sz, c_vp], ctypes.c_int),
-            "sva_kv4_write": ([ctypes.POINTER(Kv4CacheArgs), c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64,
+            "sva_prompt_attention_workspace_size": ([c_vp], c_sz),
+            "sva_prompt_attention": ([c_vp, c_vp, c_sz, c_vp], ctypes.c_int),
+            "sva_kv4_write": ([c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64,
                                c_i32, c_i32, c_i64, c_vp, c_vp, c_vp], ctypes.c_int),
-            "sva_kv4_read": ([ctypes.POINTER(Kv4CacheArgs), c_vp, c_vp, c_i32, c_i32, c_i64, c_vp, c_vp],
+            "sva_kv4_read": ([c_vp, c_vp, c_vp, c_i32, c_i32, c_i64, c_vp, c_vp],
                              ctypes.c_int),
-            "sva_kv4_decode_workspace_size": ([ctypes.POINTER(Kv4CacheArgs), ctypes.POINTER(Kv4DecodeArgs)], c_sz),
-            "sva_kv4_decode": ([ctypes.POINTER(Kv4CacheArgs), ctypes.POINTER(Kv4DecodeArgs), c_vp, c_sz, c_vp],
+            "sva_kv4_decode_workspace_size": ([c_vp, c_vp], c_sz),
+            "sva_kv4_decode": ([c_vp, c_vp, c_vp, c_sz, c_vp],
                                ctypes.c_int),
-            "sva_cache_evict_workspace_size": ([ctypes.POINTER(EvictArgs)], c_sz),
-            "sva_cache_evict": ([ctypes.POINTER(EvictArgs), ctypes.POINTER(EvictArray), c_vp, c_sz, c_vp],
+            "sva_cache_evict_workspace_size": ([c_vp], c_sz),
+            "sva_cache_evict": ([c_vp, c_vp, c_vp, c_sz, c_vp],
                                 ctypes.c_int),
         }
         for name, (argtypes, restype) in sigs.items():

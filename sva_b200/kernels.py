@@ -582,22 +582,32 @@ def top_unique(candidate_idx: torch.Tensor, candidate_scores: torch.Tensor, cand
 # ------------------------------------------------------------------------------------------
 
 
-def _same_device(dev: torch.device, **tensors: torch.Tensor | None) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            if not t.is_cuda:
-                _cuda(t, name)
-            raise ValueError(f"{name} is on {t.device}, the call's other tensors on {dev}")
+# The host's share of these calls is of the order of the smallest kernels' time, so arguments are checked and packed
+# with few interpreter steps: device numbers instead of device objects, one stride() a tensor, packed bytes.
+_pack_prompt = _lib.packer(_lib.PromptArgs).pack
+_pack_cache = _lib.packer(_lib.Kv4CacheArgs).pack
+_pack_decode = _lib.packer(_lib.Kv4DecodeArgs).pack
+_pack_evict = _lib.packer(_lib.EvictArgs).pack
+_pack_row = _lib.packer(_lib.EvictArray).pack
 
 
-def _call(dev: torch.device, fn, *args) -> None:
-    """fn(*args, stream) with ``dev`` as the current device, on its current stream."""
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+def _there(index: int, t: torch.Tensor, name: str) -> int:
+    """The data pointer of a tensor of the call, which has to be on CUDA device ``index``."""
+    if t.get_device() != index:
+        _cuda(t, name)
+        raise ValueError(f"{name} is on {t.device}, the call's other tensors on cuda:{index}")
+    return t.data_ptr()
+
+
+def _call(index: int, fn, *args) -> None:
+    """fn(*args, stream) with device ``index`` current, on its current stream."""
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc)
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != _lib.SVA_OK:
+        _lib.check(rc)
 
 
 def _scratch(dev: torch.device, nbytes: int) -> torch.Tensor | None:
@@ -606,19 +616,27 @@ def _scratch(dev: torch.device, nbytes: int) -> torch.Tensor | None:
     return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
 
 
-def _int64(t: torch.Tensor, name: str, n: int) -> int:
-    if t.dtype != torch.int64 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+def _int64(index: int, t: torch.Tensor, name: str, n: int) -> int:
+    if t.dtype != torch.int64 or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int64 tensor of {n} entries")
-    return t.data_ptr()
+    return _there(index, t, name)
 
 
-def _page_table(t: torch.Tensor | None, n_seqs: int) -> tuple:
+def _flag(index: int, t: torch.Tensor | None) -> int:
+    if t is None:
+        return 0
+    if t.dtype != torch.int32 or t.numel() != 1:
+        raise ValueError("status must be an int32 tensor of one entry")
+    return _there(index, t, "status")
+
+
+def _page_table(index: int, t: torch.Tensor | None, n_seqs: int, name: str = "page_table") -> tuple:
     """(pointer, row stride, columns) of a page table, or of none."""
     if t is None:
-        return None, 0, 0
+        return 0, 0, 0
     if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != n_seqs or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"page_table must be an int32 [{n_seqs}, max_pages] tensor with contiguous rows")
-    return t.data_ptr(), t.stride(0), t.shape[1]
+        raise ValueError(f"{name} must be an int32 [{n_seqs}, max_pages] tensor with contiguous rows")
+    return _there(index, t, name), t.stride(0), t.shape[1]
 
 
 def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, cu_seqlens: torch.Tensor, *,
@@ -627,7 +645,7 @@ def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     """Attention over whole prompts packed without padding (sva_prompt_attention).
 
     q [N, H, D]; keys / values [Nk, Hkv, D] (any strides with contiguous rows; H a multiple of Hkv, D <= 256);
-    ``cu_seqlens`` [B + 1] int64 on the device: sequence b owns query rows cu_seqlens[b] ..
+    ``cu_seqlens`` [B + 1] int64 on the device, not decreasing: sequence b owns query rows cu_seqlens[b] ..
     cu_seqlens[b + 1] - 1, and key rows likewise by ``cu_seqlens_k`` (None: the same).  With Lq query and Lk key
     rows, query i sees keys j <= i + Lk - Lq, so new tokens may follow a cached beginning; ``causal``
     False: all Lk.  A query that sees no key gets zeros; rows behind the last sequence are left as they
@@ -635,38 +653,42 @@ def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     rows of D <= 128 channels, a multiple of 8, run on the tensor cores when every stride is a multiple of 16
     bytes; other calls on the CUDA cores in fp32.  ``status`` (int32 device scalar) receives a timeout flag.
     """
-    _cuda(q, "q")
-    dev = q.device
-    _same_device(dev, keys=keys, values=values, cu_seqlens=cu_seqlens, cu_seqlens_k=cu_seqlens_k, out=out, status=status)
-    if q.dim() != 3 or keys.dim() != 3 or values.shape != keys.shape or keys.shape[2] != q.shape[2]:
+    if not q.is_cuda:
+        _cuda(q, "q")
+    index = q.get_device()
+    dtype = q.dtype
+    if q.dim() != 3 or keys.dim() != 3 or values.shape != keys.shape:
         raise ValueError("prompt_attention takes q [N, H, D] and keys / values [Nk, Hkv, D]")
-    if keys.dtype != q.dtype or values.dtype != q.dtype:
+    if keys.dtype != dtype or values.dtype != dtype:
         raise TypeError("q, keys and values must share a dtype")
     n, n_heads, head_dim = q.shape
-    if head_dim > 1 and (q.stride(2) != 1 or keys.stride(2) != 1 or values.stride(2) != 1):
+    nk, n_kv, key_dim = keys.shape
+    (qr, qh, q1), (kr, kh, k1), (vr, vh, v1) = q.stride(), keys.stride(), values.stride()
+    if key_dim != head_dim:
+        raise ValueError("q and keys must share their last dimension")
+    if head_dim > 1 and not q1 == k1 == v1 == 1:
         raise ValueError("q, keys and values must have contiguous rows")
     n_seqs = cu_seqlens.shape[0] - 1 if cu_seqlens.dim() == 1 else -1
     if n_seqs < 0:
         raise ValueError("cu_seqlens must be a [B + 1] tensor")
-    if cu_seqlens_k is None and keys.shape[0] != n:
+    if cu_seqlens_k is None and nk != n:
         raise ValueError("cu_seqlens_k is needed where queries and keys differ in number")
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != q.shape or out.dtype != q.dtype or (head_dim > 1 and out.stride(2) != 1):
+        out = torch.empty((n, n_heads, head_dim), dtype=dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != dtype or (head_dim > 1 and out.stride(2) != 1):
         raise ValueError("out must have q's shape and dtype, with contiguous rows")
-    lse = torch.full((n_heads, n), float("-inf"), dtype=torch.float32, device=dev) if want_lse else None
-    a = _lib.PromptArgs(n_seqs, n_heads, keys.shape[1], head_dim, dtype_code(q.dtype), int(causal),
-                        head_dim ** -0.5 if softmax_scale is None else softmax_scale, n, keys.shape[0],
-                        q.data_ptr(), q.stride(0), q.stride(1), keys.data_ptr(), keys.stride(0), keys.stride(1),
-                        values.data_ptr(), values.stride(0), values.stride(1),
-                        _int64(cu_seqlens, "cu_seqlens", n_seqs + 1),
-                        None if cu_seqlens_k is None else _int64(cu_seqlens_k, "cu_seqlens_k", n_seqs + 1),
-                        out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse), _ptr(status))
+    lse = torch.full((n_heads, n), float("-inf"), dtype=torch.float32, device=q.device) if want_lse else None
+    a = _pack_prompt(n_seqs, n_heads, n_kv, head_dim, dtype_code(dtype), 1 if causal else 0,
+                     head_dim ** -0.5 if softmax_scale is None else softmax_scale, n, nk, q.data_ptr(), qr, qh,
+                     _there(index, keys, "keys"), kr, kh, _there(index, values, "values"), vr, vh,
+                     _int64(index, cu_seqlens, "cu_seqlens", n_seqs + 1),
+                     0 if cu_seqlens_k is None else _int64(index, cu_seqlens_k, "cu_seqlens_k", n_seqs + 1),
+                     _there(index, out, "out"), out.stride(0), out.stride(1), 0 if lse is None else lse.data_ptr(),
+                     _flag(index, status))
     lib = _lib.load()
-    ref = ctypes.byref(a)
-    nbytes = lib.sva_prompt_attention_workspace_size(ref)
-    ws = _scratch(dev, nbytes)
-    _call(dev, lib.sva_prompt_attention, ref, _ptr(ws), nbytes)
+    nbytes = lib.sva_prompt_attention_workspace_size(a)
+    ws = _scratch(q.device, nbytes)
+    _call(index, lib.sva_prompt_attention, a, _ptr(ws), nbytes)
     return (out, lse) if want_lse else out
 
 
@@ -691,20 +713,22 @@ def kv4_empty(pages: int, n_kv_heads: int, rows: int, head_dim: int, device="cud
                       for tail, dtype in (((head_dim // 2,), torch.uint8), ((head_dim // 32, 2), torch.bfloat16)) * 2))
 
 
-def _kv4_args(cache: Kv4Cache, n_seqs: int, page_table: torch.Tensor | None) -> _lib.Kv4CacheArgs:
+def _kv4_args(index: int, cache: Kv4Cache, n_seqs: int, page_table: torch.Tensor | None) -> tuple:
+    """The packed sva_kv4_cache, kv heads, head_dim and the rows that a sequence can have."""
     kc, kp, vc, vp = cache
-    dev = _cuda(kc, "k_codes").device
-    _same_device(dev, k_params=kp, v_codes=vc, v_params=vp, page_table=page_table)
-    if kc.dim() != 4 or kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or vc.shape != kc.shape:
+    shape = kc.shape
+    if len(shape) != 4 or kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or vc.shape != shape:
         raise ValueError("codes must be uint8 [pages, Hkv, rows, D / 2]")
-    pages, n_kv, rows, half = kc.shape
+    pages, n_kv, rows, half = shape
     tail = (pages, n_kv, rows, half // 16, 2)
     if kp.dtype != torch.bfloat16 or vp.dtype != torch.bfloat16 or kp.shape != tail or vp.shape != tail:
         raise ValueError("parameters must be bfloat16 [pages, Hkv, rows, D / 32, 2]")
     if not (kc.is_contiguous() and kp.is_contiguous() and vc.is_contiguous() and vp.is_contiguous()):
         raise ValueError("the cache's tensors must be contiguous")
-    return _lib.Kv4CacheArgs(pages, rows, n_kv, half * 2, kc.data_ptr(), kp.data_ptr(), vc.data_ptr(), vp.data_ptr(),
-                             *_page_table(page_table, n_seqs))
+    table, stride, cols = _page_table(index, page_table, n_seqs)
+    c = _pack_cache(pages, rows, n_kv, half * 2, _there(index, kc, "k_codes"), _there(index, kp, "k_params"),
+                    _there(index, vc, "v_codes"), _there(index, vp, "v_params"), table, stride, cols)
+    return c, n_kv, half * 2, rows * cols if table else rows
 
 
 def kv4_write(keys: torch.Tensor, values: torch.Tensor, cache: Kv4Cache, start: torch.Tensor, *,
@@ -714,46 +738,53 @@ def kv4_write(keys: torch.Tensor, values: torch.Tensor, cache: Kv4Cache, start: 
     keys / values [B, Hkv, T, D]: token t of sequence b goes to position start[b] + t; or packed
     [N, Hkv, D] with ``cu_seqlens`` [B + 1]: row n of sequence b goes to start[b] + n - cu_seqlens[b], and rows of no
     sequence are skipped.  ``start`` [B] int64 on the device, so that a captured graph may append at a moving
-    position.  Positions outside the cache are skipped.
+    position.  Positions outside the cache are skipped; no two rows of a call may meet at one cache row.
     """
-    _cuda(keys, "keys")
+    if not keys.is_cuda:
+        _cuda(keys, "keys")
+    index = keys.get_device()
+    shape = keys.shape
     packed = cu_seqlens is not None
-    if keys.dim() != (3 if packed else 4) or values.shape != keys.shape:
+    if len(shape) != (3 if packed else 4) or values.shape != shape:
         raise ValueError("kv4_write takes keys and values [B, Hkv, T, D], or [N, Hkv, D] with cu_seqlens")
     if values.dtype != keys.dtype:
         raise TypeError("keys and values must share a dtype")
-    dev = keys.device
-    _same_device(dev, values=values, start=start, cu_seqlens=cu_seqlens, k_codes=cache.k_codes)
-    if keys.stride(-1) != 1 or values.stride(-1) != 1:
+    ks, vs = keys.stride(), values.stride()
+    if ks[-1] != 1 or vs[-1] != 1:
         raise ValueError("keys and values must have contiguous rows")
     n_seqs = start.shape[0] if start.dim() == 1 else -1
-    c = _kv4_args(cache, n_seqs, page_table)
-    if keys.shape[1] != c.n_kv_heads or keys.shape[-1] != c.head_dim or (not packed and keys.shape[0] != n_seqs):
+    c, n_kv, head_dim, _ = _kv4_args(index, cache, n_seqs, page_table)
+    if shape[1] != n_kv or shape[-1] != head_dim or (not packed and shape[0] != n_seqs):
         raise ValueError("keys do not match the cache's heads, head_dim or start's sequences")
-    order = (lambda t: (0, t.stride(1), t.stride(0))) if packed else (lambda t: t.stride()[:3])
+    at = _int64(index, start, "start", n_seqs)
+    cu = _int64(index, cu_seqlens, "cu_seqlens", n_seqs + 1) if packed else 0
+    kp, vp, code = keys.data_ptr(), _there(index, values, "values"), dtype_code(keys.dtype)
     if n_seqs == 0 or keys.numel() == 0:
         return
-    _call(dev, _lib.load().sva_kv4_write, ctypes.byref(c), keys.data_ptr(), *order(keys), values.data_ptr(),
-          *order(values), dtype_code(keys.dtype), n_seqs, keys.shape[0] if packed else keys.shape[2],
-          _int64(start, "start", n_seqs), None if cu_seqlens is None else _int64(cu_seqlens, "cu_seqlens", n_seqs + 1))
+    if packed:
+        _call(index, _lib.load().sva_kv4_write, c, kp, 0, ks[1], ks[0], vp, 0, vs[1], vs[0], code, n_seqs, shape[0], at, cu)
+    else:
+        _call(index, _lib.load().sva_kv4_write, c, kp, ks[0], ks[1], ks[2], vp, vs[0], vs[1], vs[2], code, n_seqs,
+              shape[2], at, 0)
 
 
 def kv4_read(cache: Kv4Cache, start: torch.Tensor, count: int, *, dtype: torch.dtype = torch.bfloat16,
              page_table: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Positions start[b] .. start[b] + count - 1 of every sequence back in ``dtype`` (sva_kv4_read): keys and
     values [B, Hkv, count, D]; zeros where a position lies outside the cache.  ``start`` [B] int64, device."""
-    dev = _cuda(cache.k_codes, "k_codes").device
-    _same_device(dev, start=start)
+    if not cache[0].is_cuda:
+        _cuda(cache[0], "k_codes")
+    index = cache[0].get_device()
     n_seqs = start.shape[0] if start.dim() == 1 else -1
-    c = _kv4_args(cache, n_seqs, page_table)
+    c, n_kv, head_dim, _ = _kv4_args(index, cache, n_seqs, page_table)
     if count < 0:
         raise ValueError("count must not be negative")
-    code = dtype_code(dtype)
-    out = torch.empty(2, n_seqs, c.n_kv_heads, count, c.head_dim, dtype=dtype, device=dev)
-    if out.numel() > 0:
-        _call(dev, _lib.load().sva_kv4_read, ctypes.byref(c), out[0].data_ptr(), out[1].data_ptr(), code, n_seqs, count,
-              _int64(start, "start", n_seqs))
-    return out[0], out[1]
+    code, at = dtype_code(dtype), _int64(index, start, "start", n_seqs)
+    shape = (n_seqs, n_kv, count, head_dim)
+    k, v = torch.empty(shape, dtype=dtype, device=start.device), torch.empty(shape, dtype=dtype, device=start.device)
+    if k.numel() > 0:
+        _call(index, _lib.load().sva_kv4_read, c, k.data_ptr(), v.data_ptr(), code, n_seqs, count, at)
+    return k, v
 
 
 def kv4_decode(q: torch.Tensor, cache: Kv4Cache, *, seq_lens: torch.Tensor | None = None,
@@ -769,48 +800,58 @@ def kv4_decode(q: torch.Tensor, cache: Kv4Cache, *, seq_lens: torch.Tensor | Non
     goes by these sums).  Returns out [B, H, T, D] (and the log-sum-exp [B, H, T] fp32 with ``want_lse``).
     A token that sees no key gets zeros.
     """
-    _cuda(q, "q")
-    dev = q.device
-    if q.dim() != 4:
+    if not q.is_cuda:
+        _cuda(q, "q")
+    index = q.get_device()
+    shape = q.shape
+    if len(shape) != 4:
         raise ValueError("kv4_decode takes q [B, H, T, D]")
-    n_seqs, n_heads, n_tokens, head_dim = q.shape
-    _same_device(dev, k_codes=cache.k_codes, seq_lens=seq_lens, out=out, weights=weights, status=status)
-    c = _kv4_args(cache, n_seqs, page_table)
-    if head_dim != c.head_dim or q.stride(3) != 1:
+    n_seqs, n_heads, n_tokens, head_dim = shape
+    c, n_kv, cache_dim, capacity = _kv4_args(index, cache, n_seqs, page_table)
+    qs = q.stride()
+    if head_dim != cache_dim or qs[3] != 1:
         raise ValueError("q must have contiguous rows of the cache's head_dim")
     if max_len is None:
-        max_len = c.page_rows * (c.page_table_cols if page_table is not None else 1)
+        max_len = capacity
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    elif out.shape != shape or out.dtype != q.dtype or out.stride(3) != 1:
         raise ValueError("out must have q's shape and dtype, with contiguous rows")
-    if weights is not None and (weights.dtype != torch.float32 or weights.dim() != 3 or weights.stride(2) != 1
-                                or weights.shape[:2] != (n_seqs, c.n_kv_heads) or weights.shape[2] < max_len):
-        raise ValueError("weights must be float32 [B, Hkv, >= max_len] with contiguous rows")
-    lse = torch.empty(n_seqs, n_heads, n_tokens, dtype=torch.float32, device=dev) if want_lse else None
-    a = _lib.Kv4DecodeArgs(n_seqs, n_heads, n_tokens, dtype_code(q.dtype), max_len,
-                           head_dim ** -0.5 if softmax_scale is None else softmax_scale, q.data_ptr(), *q.stride()[:3],
-                           None if seq_lens is None else _int64(seq_lens, "seq_lens", n_seqs), out.data_ptr(),
-                           *out.stride()[:3], _ptr(lse), _ptr(weights),
-                           *((0, 0) if weights is None else weights.stride()[:2]), _ptr(status))
+    os = out.stride()
+    wp = ws = wh = 0
+    if weights is not None:
+        if (weights.dtype != torch.float32 or weights.dim() != 3 or weights.stride(2) != 1
+                or weights.shape[:2] != (n_seqs, n_kv) or weights.shape[2] < max_len):
+            raise ValueError("weights must be float32 [B, Hkv, >= max_len] with contiguous rows")
+        wp, (ws, wh, _) = _there(index, weights, "weights"), weights.stride()
+    lse = torch.empty(n_seqs, n_heads, n_tokens, dtype=torch.float32, device=q.device) if want_lse else None
+    a = _pack_decode(n_seqs, n_heads, n_tokens, dtype_code(q.dtype), max_len,
+                     head_dim ** -0.5 if softmax_scale is None else softmax_scale, q.data_ptr(), qs[0], qs[1], qs[2],
+                     0 if seq_lens is None else _int64(index, seq_lens, "seq_lens", n_seqs), _there(index, out, "out"),
+                     os[0], os[1], os[2], 0 if lse is None else lse.data_ptr(), wp, ws, wh, _flag(index, status))
     if q.numel() > 0:
         lib = _lib.load()
-        refs = ctypes.byref(c), ctypes.byref(a)
-        nbytes = lib.sva_kv4_decode_workspace_size(*refs)
-        ws = _scratch(dev, nbytes)
-        _call(dev, lib.sva_kv4_decode, *refs, _ptr(ws), nbytes)
+        nbytes = lib.sva_kv4_decode_workspace_size(c, a)
+        scratch = _scratch(q.device, nbytes)
+        _call(index, lib.sva_kv4_decode, c, a, _ptr(scratch), nbytes)
     return (out, lse) if want_lse else out
 
 
-def _span(t: torch.Tensor) -> tuple[int, int]:
-    """First byte of a tensor and the byte behind its last."""
-    first = t.data_ptr()
-    return first, first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 < b1 and b0 < a1
+def _rows_span(t: torch.Tensor, name: str) -> tuple:
+    """(first byte, byte behind the last, page stride, head stride, row bytes) of [pages, heads, rows, ...] with
+    contiguous rows."""
+    shape, size = t.shape, t.element_size()
+    if len(shape) < 3:
+        raise ValueError(f"{name} must be [pages, Hkv, page_rows, ...] tensors")
+    if t.is_contiguous():
+        row = t.stride(2) * size
+    else:
+        row = math.prod(shape[3:]) * size
+        if 0 not in shape and not t[0, 0].is_contiguous():
+            raise ValueError(f"{name} must have contiguous rows")
+    page, head = t.stride(0) * size, t.stride(1) * size
+    at = t.data_ptr()
+    return at, at + (shape[0] - 1) * page + (shape[1] - 1) * head + shape[2] * row, page, head, row
 
 
 def cache_evict(rows: Sequence[torch.Tensor], weights: torch.Tensor, seq_lens: torch.Tensor, keep: int, *,
@@ -828,8 +869,9 @@ def cache_evict(rows: Sequence[torch.Tensor], weights: torch.Tensor, seq_lens: t
     -1 padded; lengths [B] int64).  Append new rows at the returned lengths, and keep the model's own position
     count for rotary embeddings: rows are not re-rotated.
     """
-    _cuda(weights, "weights")
-    dev = weights.device
+    if not weights.is_cuda:
+        _cuda(weights, "weights")
+    index, dev = weights.get_device(), weights.device
     in_place = out is None
     if in_place and (out_weights is not None or out_page_table is not None):
         raise ValueError("out_weights and out_page_table go with out")
@@ -839,42 +881,47 @@ def cache_evict(rows: Sequence[torch.Tensor], weights: torch.Tensor, seq_lens: t
     dst = src if in_place else list(out)
     if not 1 <= len(src) <= _lib.EVICT_MAX_ARRAYS or len(dst) != len(src):
         raise ValueError("cache_evict takes 1 to 8 row tensors, and as many outputs")
+    if keep < 0:
+        raise ValueError("keep must not be negative")
     dst_weights = weights if in_place else out_weights
     dst_table = page_table if in_place else out_page_table
     n_seqs = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
-    n_kv = src[0].shape[1] if src[0].dim() >= 3 else -1
-    _same_device(dev, seq_lens=seq_lens, page_table=page_table, out_weights=dst_weights, out_page_table=dst_table)
+    like, like_out = src[0].shape[:3], dst[0].shape[:3]
+    spans, packed = [], []
+    for s, d in zip(src, dst):
+        one = _rows_span(s, "rows")
+        two = one if in_place else _rows_span(d, "out")
+        if s.shape[:3] != like or d.shape[:3] != like_out:
+            raise ValueError("rows must agree in their first three dimensions, and so must out")
+        if not in_place and (s.dtype != d.dtype or s.shape[3:] != d.shape[3:]):
+            raise ValueError("out must have rows of the same shape and dtype")
+        if _there(index, s, "rows") and _there(index, d, "out"):
+            spans.append((one, two))
+        packed.append(_pack_row(one[0], two[0], one[4], one[2], one[3], two[2], two[3]))
+    n_kv = like[1]
     for name, w in (("weights", weights), ("out_weights", dst_weights)):
         if w.dtype != torch.float32 or w.dim() != 3 or w.shape[:2] != (n_seqs, n_kv) or w.stride(2) != 1:
             raise ValueError(f"{name} must be float32 [B, Hkv, width] with contiguous rows")
-    arrays = (_lib.EvictArray * len(src))()
-    for i, (s, d) in enumerate(zip(src, dst)):
-        _same_device(dev, rows=s, out=d)
-        for t, like in ((s, src[0]), (d, dst[0])):
-            if t.dim() < 3 or t.shape[:3] != like.shape[:3] or t.shape[1] != n_kv or not t[0, 0].is_contiguous():
-                raise ValueError("rows must be [pages, Hkv, page_rows, ...] tensors of one shape with contiguous rows")
-        if s.dtype != d.dtype or s.shape[3:] != d.shape[3:]:
-            raise ValueError("out must have rows of the same shape and dtype")
-        if not in_place and (any(_overlap(d, t) for t in src) or any(_overlap(d, t) for t in dst[:i])):
-            raise ValueError("out must not overlap rows or itself")
-        size = s.element_size()
-        arrays[i] = (s.data_ptr(), d.data_ptr(), math.prod(s.shape[3:]) * size, s.stride(0) * size, s.stride(1) * size,
-                     d.stride(0) * size, d.stride(1) * size)
-    if not in_place and _overlap(weights, dst_weights):
-        raise ValueError("out_weights must not overlap weights")
-    kept = torch.empty(n_seqs, n_kv, max(keep, 0), dtype=torch.int32, device=dev)
-    lens = torch.empty(n_seqs, dtype=torch.int64, device=dev)
-    rows_of = (lambda t, table: t.shape[2] * (table.shape[1] if table is not None else 1))
-    a = _lib.EvictArgs(n_seqs, n_kv, len(src), int(in_place), min(weights.shape[2], rows_of(src[0], page_table)), keep, recent,
-                       _int64(seq_lens, "seq_lens", n_seqs), weights.data_ptr(), weights.stride(0), weights.stride(1),
-                       dst_weights.data_ptr(), dst_weights.stride(0), dst_weights.stride(1), dst_weights.shape[2],
-                       src[0].shape[0], src[0].shape[2], dst[0].shape[0], dst[0].shape[2],
-                       *_page_table(page_table, n_seqs), *_page_table(dst_table, n_seqs), kept.data_ptr(),
-                       lens.data_ptr())
+    if not in_place:
+        w, ow = _rows_span(weights.unsqueeze(3), "weights"), _rows_span(dst_weights.unsqueeze(3), "out_weights")
+        read, written = [one for one, _ in spans] + [w], [two for _, two in spans] + [ow]
+        for i, d in enumerate(written):
+            for other in read + written[:i]:
+                if d[0] < other[1] and other[0] < d[1]:
+                    raise ValueError("out and out_weights must not overlap rows, weights or one another")
+    kept = torch.empty((n_seqs, n_kv, keep), dtype=torch.int32, device=dev)
+    lens = torch.empty((n_seqs,), dtype=torch.int64, device=dev)
+    table, table_stride, cols = _page_table(index, page_table, n_seqs)
+    to, to_stride, to_cols = _page_table(index, dst_table, n_seqs, "out_page_table")
+    width = weights.shape[2]
+    a = _pack_evict(n_seqs, n_kv, len(src), 1 if in_place else 0, min(width, like[2] * (cols if table else 1)), keep, recent,
+                    _int64(index, seq_lens, "seq_lens", n_seqs), weights.data_ptr(), weights.stride(0), weights.stride(1),
+                    _there(index, dst_weights, "out_weights"), dst_weights.stride(0), dst_weights.stride(1),
+                    dst_weights.shape[2], like[0], like[2], like_out[0], like_out[2], table, table_stride, cols, to,
+                    to_stride, to_cols, kept.data_ptr(), lens.data_ptr())
     if n_seqs > 0:
         lib = _lib.load()
-        ref = ctypes.byref(a)
-        nbytes = lib.sva_cache_evict_workspace_size(ref)
+        nbytes = lib.sva_cache_evict_workspace_size(a)
         ws = _scratch(dev, nbytes)
-        _call(dev, lib.sva_cache_evict, ref, arrays, _ptr(ws), nbytes)
+        _call(index, lib.sva_cache_evict, a, b"".join(packed), _ptr(ws), nbytes)
     return kept, lens
