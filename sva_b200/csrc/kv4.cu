@@ -305,27 +305,78 @@ __device__ __forceinline__ uint32_t codes_bf16(uint32_t v) {
 
 __device__ __forceinline__ int slot_key(int r) { return (r & 8) + ((r & 7) >> 1) + 4 * (r & 1); }
 
-template <typename T, int D, int NT>
+__device__ __forceinline__ void mma_f16(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// A word's eight codes around 8 as the pairs (i, i + 4), i = 0..3, of a score operand: in fp16 for 16-bit queries, where two of
+// the four pairs need no shift (9 instructions a word), in bf16 for fp32 queries, whose three bf16 parts keep every bit.
+template <bool kHalf>
+__device__ __forceinline__ void code_fragments(uint32_t w, uint32_t r[4]) {
+  if constexpr (kHalf) {
+    // 0x6400 is 1024: 1024 + c from the low nibbles, 1024 + 16 c from the high ones
+    const uint32_t u = w >> 8;
+    const uint32_t x[4] = {(w & 0x000F000Fu) | 0x64006400u, (w & 0x00F000F0u) | 0x64006400u,
+                           (u & 0x000F000Fu) | 0x64006400u, (u & 0x00F000F0u) | 0x64006400u};
+    const __half2 k1032 = __half2half2(__ushort_as_half(0x6408)), k16 = __half2half2(__ushort_as_half(0x2C00)),
+                  k72 = __half2half2(__ushort_as_half(0xD480));  // 1032, 1/16, -72
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = reinterpret_cast<const __half2&>(x[i]);
+      const __half2 d = i & 1 ? __hfma2(h, k16, k72) : __hsub2(h, k1032);
+      r[i] = reinterpret_cast<const uint32_t&>(d);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = codes_bf16(w >> (4 * i));
+  }
+}
+
+// KP: key tiles that share the 8 columns of an accumulator.  With at most 4 query columns, columns 0-3 take one 16-key
+// tile and 4-7 the next (each with the other's query columns zero), so that no lane's softmax work is for nothing.
+template <typename T, int D, int NT, int KP>
 struct DecShape {
   static constexpr bool kWide = sizeof(T) == 4;
-  static constexpr int kQParts = kWide ? 3 : (std::is_same<T, __half>::value ? 2 : 1);  // bf16 parts of q: exact
-  static constexpr int kPParts = kWide ? 3 : 1;
+  static constexpr int kQParts = kWide ? 3 : 1;                                          // bf16 parts of q
+  static constexpr int kPParts = kWide ? 3 : (std::is_same<T, __half>::value ? 2 : 1);  // and of p s
   static constexpr int kGroups = D / kGroup;
   static constexpr int kTileBytes = kTileKeys * (D / 2 + D / 8) * 2;
-  static constexpr int kStages = D == 64 ? 3 : 2;
-  static constexpr int kCols = 8 * NT;
+  static constexpr int kStages = 2;
+  static constexpr int kCols = KP == 2 ? 4 : 8 * NT;
   static constexpr int kSmem = kDecWarps * kStages * kTileBytes + 128;
 };
 
-template <typename T, int D, int NT, bool kLogits>
+template <int N>
+__device__ __forceinline__ void load_params(const unsigned char* at, uint32_t (&v)[N]) {
+  if constexpr (N == 2) {
+    const uint2 x = *reinterpret_cast<const uint2*>(at);
+    v[0] = x.x, v[1] = x.y;
+  } else {
+    const uint4 x = *reinterpret_cast<const uint4*>(at);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+  }
+}
+
+template <typename T, int D, int NT, int KP, bool kLogits>
 __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4DecParams p) {
-  using S = DecShape<T, D, NT>;
-  constexpr int kG = S::kGroups, kStages = S::kStages;
+  using S = DecShape<T, D, NT, KP>;
+  static_assert(KP == 1 || NT == 1, "shared accumulators hold one column tile");
+  constexpr int kG = S::kGroups, kStages = S::kStages, kSlots = 4 / KP;
+  constexpr bool kHalf = !S::kWide;
   extern __shared__ __align__(128) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int ct = blockIdx.y % p.col_tiles, h = blockIdx.y / p.col_tiles, b = blockIdx.z;
   const int chunk = blockIdx.x;
   const int col0 = ct * S::kCols;
+  pdl_launch_dependents();
   const int64_t len = seq_len_of(p, b);
   const int64_t key0 = chunk * p.chunk_keys, key1 = min(len, key0 + p.chunk_keys);
   if (key0 >= len && chunk > 0) return;  // the join reads ceil(len / chunk_keys) chunks (at least one)
@@ -346,14 +397,14 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
     const int i = it0 + lane;
     return i < my_tiles ? p.c.row(b, h, key0 + (int64_t)(warp + i * kDecWarps) * kTileKeys) : -1;
   };
-  int64_t rows_cur = rows_of(0), rows_next = rows_of(32);
+  int64_t rows_cur = rows_of(0), rows_next = my_tiles > 32 ? rows_of(32) : -1;
+  constexpr uint32_t kC = kTileKeys * D / 2, kP = kTileKeys * D / 8;  // bytes of a tile's codes and parameters
   auto issue = [&](int it, int base) {  // copies of tile it into stage it % kStages; base: first tile of rows_cur
     const int64_t r = it < base + 32 ? __shfl_sync(0xFFFFFFFFu, rows_cur, it - base)
                                      : __shfl_sync(0xFFFFFFFFu, rows_next, it - base - 32);
     if (lane == 0) {
       const int s = it % kStages;
       const uint32_t bar = bar0 + 8 * s, dst = smem_u32(ring + s * S::kTileBytes);
-      constexpr uint32_t kC = kTileKeys * D / 2, kP = kTileKeys * D / 8;
       if (r >= 0) {
         mbar_expect_tx(bar, S::kTileBytes);
         bulk_load(dst, p.c.k_codes + r * (D / 2), kC, bar);
@@ -369,49 +420,76 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
   for (int s = 0; s < kStages; ++s)
     if (s < my_tiles) issue(s, 0);
 
-  // query fragments: column g of every 8-column tile, channels 32 G + 8 t .. + 7, pairs (i, i + 4)
-  uint32_t qf[kG][S::kQParts][NT][4];
-  float qsum[kG][NT][2];
+  // query fragments: the lane's column (g, or g % 4), channels 32 G + 8 t .. + 7, pairs (i, i + 4).  16-bit queries are
+  // scaled by a power of two that brings a column's largest element into [1, 2): exact in fp16, but for what lies
+  // 2^-14 below the largest, which is off by at most 2^-25 of it.
+  uint32_t qf[kG][S::kQParts][KP][NT][4];
+  float qsum[kG][NT][2], scale[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int col = col0 + 8 * n + g;
+    const int col = col0 + (KP == 2 ? (g & 3) : 8 * n + g);
     const bool live = col < p.n_cols;
     const int tok = col / p.groups, head = h * p.groups + col % p.groups;
     const T* src = reinterpret_cast<const T*>(p.q) + b * p.q_seq + (int64_t)head * p.q_head + (int64_t)tok * p.q_row;
+    float x[kG][8], big = 0.f, unit = 1.f;
 #pragma unroll
-    for (int gr = 0; gr < kG; ++gr) {
-      float x[8], sum = 0.f;
+    for (int gr = 0; gr < kG; ++gr)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] = live ? to_f32<T>(src[gr * kGroup + 8 * t + i]) : 0.f;
-        sum += x[i];
+        x[gr][i] = live ? to_f32<T>(src[gr * kGroup + 8 * t + i]) : 0.f;
+        big = fmaxf(big, fabsf(x[gr][i]));
       }
+    if constexpr (kHalf) {
+      big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
+      const uint32_t e = min(max(__float_as_uint(big) >> 23, 1u), 253u);
+      unit = __uint_as_float(e << 23);
+      const float down = __uint_as_float((254u - e) << 23);
+#pragma unroll
+      for (int gr = 0; gr < kG; ++gr)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[gr][i] *= down;
+    }
+    // this lane accumulates columns 2t and 2t + 1 (mod 4)
+    const int c = KP == 2 ? 2 * (t & 1) : 2 * t;
+    scale[n][0] = p.scale_log2 * __shfl_sync(0xFFFFFFFFu, unit, c * 4);
+    scale[n][1] = p.scale_log2 * __shfl_sync(0xFFFFFFFFu, unit, (c + 1) * 4);
+#pragma unroll
+    for (int gr = 0; gr < kG; ++gr) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += x[gr][i];
       sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
       sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-      // this lane accumulates columns 2t and 2t + 1
-      qsum[gr][n][0] = __shfl_sync(0xFFFFFFFFu, sum, (2 * t) * 4);
-      qsum[gr][n][1] = __shfl_sync(0xFFFFFFFFu, sum, (2 * t + 1) * 4);
+      qsum[gr][n][0] = __shfl_sync(0xFFFFFFFFu, sum, c * 4);
+      qsum[gr][n][1] = __shfl_sync(0xFFFFFFFFu, sum, (c + 1) * 4);
 #pragma unroll
       for (int part = 0; part < S::kQParts; ++part) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t v = pack_bf16(x[i], x[i + 4]);
-          qf[gr][part][n][i] = v;
-          x[i] -= bf16_lo(v);
-          x[i + 4] -= bf16_hi(v);
+          const uint32_t v = kHalf ? pack_f16(x[gr][i], x[gr][i + 4]) : pack_bf16(x[gr][i], x[gr][i + 4]);
+#pragma unroll
+          for (int k = 0; k < KP; ++k) qf[gr][part][k][n][i] = KP == 1 || (g >> 2) == k ? v : 0u;
+          if constexpr (S::kQParts > 1) {
+            x[gr][i] -= bf16_lo(v);
+            x[gr][i + 4] -= bf16_hi(v);
+          }
         }
       }
     }
   }
-  int limit[NT][2];  // keys that columns 2t and 2t + 1 see, counted from key0
+  int limit[NT][2];  // keys that the lane's columns see, counted from key0
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int col = col0 + 8 * n + 2 * t + j;
+      const int col = col0 + (KP == 2 ? 2 * (t & 1) : 8 * n + 2 * t) + j;
       const int64_t seen = len - p.n_tokens + col / p.groups + 1 - key0;
       limit[n][j] = col < p.n_cols ? (int)min(max(seen, (int64_t)0), p.chunk_keys) : 0;
     }
+  // keys that every column sees, and that any sees
+  const int seen_all = (int)min(max(len - p.n_tokens + 1 - key0, (int64_t)0), p.chunk_keys);
+  const int seen_any = (int)(key1 - key0);
 
   float m_run[NT][2], l_run[NT][2], zsum[kG][NT][2], acc[kG][2][NT][4];
 #pragma unroll
@@ -429,7 +507,9 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
 
   bool failed = false;
   int failed_at = 0, base = 0;
-  const int key_a = slot_key(g);
+  const int key_a = slot_key(g);                       // the lane's first key of a 16-key tile; the other is 8 behind
+  const int own = KP == 2 ? (t >> 1) * 16 + key_a : key_a;  // of a slot, for the lane's accumulator columns
+  const uint32_t byte0 = 0x4400u + 0x2222u * (g & 1), byte1 = byte0 + 0x1111u;
   for (int it = 0; it < my_tiles; ++it) {
     if (it == base + 32) {
       base += 32;
@@ -444,149 +524,174 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
     }
     const bool there = __shfl_sync(0xFFFFFFFFu, rows_cur, it - base) >= 0;
     const int l0 = (warp + it * kDecWarps) * kTileKeys;  // first key of the tile, counted from key0
-    const unsigned char* kc = ring + s * S::kTileBytes;
-    const unsigned char* kp = kc + kTileKeys * D / 2;
-    const unsigned char* vc = kp + kTileKeys * D / 8;
-    const unsigned char* vp = vc + kTileKeys * D / 2;
+    unsigned char* kc = ring + s * S::kTileBytes;
+    unsigned char* kp = kc + kC;
+    unsigned char* vc = kp + kP;
+    unsigned char* vp = vc + kC;
+    const bool whole = there && l0 + kTileKeys <= seen_all;
+    if (!whole) {
+      // parameters of keys that no column sees can be anything: make their values finite
+      const int from = there ? max(0, min(kTileKeys, seen_any - l0)) : 0;
+      for (int e = from * kG + lane; e < kTileKeys * kG; e += 32) reinterpret_cast<uint32_t*>(vp)[e] = 0u;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+    }
 
-    // scores of 64 keys x 8 NT columns
-    float sc[4][NT][4];
+    // scores of 64 keys
+    float sc[kSlots][NT][4];
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
+    for (int sl = 0; sl < kSlots; ++sl) {
+      const int k0 = sl * 16 * KP;
+      uint32_t pa[kG], pb[kG];
+      load_params<kG>(kp + (k0 + own) * (D / 8), pa);
+      load_params<kG>(kp + (k0 + own + 8) * (D / 8), pb);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[mt][n][i] = 0.f;
-      const int ka = mt * 16 + key_a, kb = ka + 8;
+        for (int i = 0; i < 4; ++i) sc[sl][n][i] = 0.f;
 #pragma unroll
       for (int gr = 0; gr < kG; ++gr) {
-        const uint32_t wa = *reinterpret_cast<const uint32_t*>(kc + ka * (D / 2) + 16 * gr + 4 * t);
-        const uint32_t wb = *reinterpret_cast<const uint32_t*>(kc + kb * (D / 2) + 16 * gr + 4 * t);
-        const uint32_t pa = *reinterpret_cast<const uint32_t*>(kp + ka * (D / 8) + 4 * gr);
-        const uint32_t pb = *reinterpret_cast<const uint32_t*>(kp + kb * (D / 8) + 4 * gr);
-        uint32_t a[2][4];
+        float c[NT][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          a[i][0] = codes_bf16(wa >> (8 * i));
-          a[i][1] = codes_bf16(wb >> (8 * i));
-          a[i][2] = codes_bf16(wa >> (8 * i + 4));
-          a[i][3] = codes_bf16(wb >> (8 * i + 4));
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) c[n][i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KP; ++k) {
+          const unsigned char* word = kc + (k0 + 16 * k + key_a) * (D / 2) + 16 * gr + 4 * t;
+          uint32_t fa[4], fb[4];
+          code_fragments<kHalf>(*reinterpret_cast<const uint32_t*>(word), fa);
+          code_fragments<kHalf>(*reinterpret_cast<const uint32_t*>(word + 8 * (D / 2)), fb);
+          const uint32_t a0[4] = {fa[0], fb[0], fa[1], fb[1]}, a1[4] = {fa[2], fb[2], fa[3], fb[3]};
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int part = 0; part < S::kQParts; ++part) {
+              const uint32_t* q = qf[gr][part][k][n];
+              if constexpr (kHalf) {
+                mma_f16(c[n], a0, q[0], q[1]);
+                mma_f16(c[n], a1, q[2], q[3]);
+              } else {
+                mma_bf16(c[n], a0, q[0], q[1]);
+                mma_bf16(c[n], a1, q[2], q[3]);
+              }
+            }
         }
-        const float sa = bf16_lo(pa), sb = bf16_lo(pb);
-        const float za = fmaf(8.f, sa, bf16_hi(pa)), zb = fmaf(8.f, sb, bf16_hi(pb));
+        const float sa = bf16_lo(pa[gr]), sb = bf16_lo(pb[gr]);
+        const float za = fmaf(8.f, sa, bf16_hi(pa[gr])), zb = fmaf(8.f, sb, bf16_hi(pb[gr]));
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float c[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int part = 0; part < S::kQParts; ++part) {
-            mma_bf16(c, a[0], qf[gr][part][n][0], qf[gr][part][n][1]);
-            mma_bf16(c, a[1], qf[gr][part][n][2], qf[gr][part][n][3]);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float sg = i < 2 ? sa : sb, zg = i < 2 ? za : zb;
-            sc[mt][n][i] = fmaf(sg, c[i], fmaf(zg, qsum[gr][n][i & 1], sc[mt][n][i]));
-          }
-        }
+          for (int i = 0; i < 4; ++i)
+            sc[sl][n][i] = fmaf(i < 2 ? sa : sb, c[n][i], fmaf(i < 2 ? za : zb, qsum[gr][n][i & 1], sc[sl][n][i]));
       }
     }
     // scale, mask, running maximum
-    float alpha[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
+      for (int sl = 0; sl < kSlots; ++sl)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int l = l0 + mt * 16 + key_a + (i < 2 ? 0 : 8);
-          const bool seen = there && l < limit[n][i & 1];
-          const float v = seen ? sc[mt][n][i] * p.scale_log2 : -INFINITY;
-          sc[mt][n][i] = v;
+          float v = sc[sl][n][i] * scale[n][i & 1];
+          const int l = l0 + sl * 16 * KP + own + (i < 2 ? 0 : 8);
+          if (!whole) v = there && l < limit[n][i & 1] ? v : -INFINITY;
+          sc[sl][n][i] = v;
           top[i & 1] = fmaxf(top[i & 1], v);
           if constexpr (kLogits) {
-            const int col = col0 + 8 * n + 2 * t + (i & 1);
-            if (col < p.n_cols && key0 + l < key1)
+            const int col = col0 + (KP == 2 ? 2 * (t & 1) : 8 * n + 2 * t) + (i & 1);
+            if (col < p.n_cols && l < seen_any)
               p.logits[(((int64_t)b * p.c.n_kv + h) * p.n_cols + col) * p.logit_stride + key0 + l] = v;
           }
         }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xFFFFFFFFu, top[j], o));
-        const float m_new = fmaxf(m_run[n][j], top[j]);
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        alpha[n][j] = ex2(m_run[n][j] - m_use);
-        m_run[n][j] = m_new;
-        l_run[n][j] *= alpha[n][j];
-        top[j] = m_use;
+        for (int o = KP == 2 ? 2 : 4; o < 32; o <<= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xFFFFFFFFu, top[j], o));
+      if (__any_sync(0xFFFFFFFFu, top[0] > m_run[n][0] || top[1] > m_run[n][1])) {
+        float alpha[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float m_new = fmaxf(m_run[n][j], top[j]);
+          alpha[j] = m_new == -INFINITY ? 0.f : ex2(m_run[n][j] - m_new);
+          m_run[n][j] = m_new;
+          l_run[n][j] *= alpha[j];
+        }
+#pragma unroll
+        for (int gr = 0; gr < kG; ++gr) {
+          zsum[gr][n][0] *= alpha[0];
+          zsum[gr][n][1] *= alpha[1];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[gr][i >> 2][n][i & 3] *= alpha[i & 1];
+        }
       }
+      const float use[2] = {m_run[n][0] == -INFINITY ? 0.f : m_run[n][0], m_run[n][1] == -INFINITY ? 0.f : m_run[n][1]};
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
+      for (int sl = 0; sl < kSlots; ++sl)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float v = ex2(sc[mt][n][i] - top[i & 1]);
-          sc[mt][n][i] = v;
+          const float v = ex2(sc[sl][n][i] - use[i & 1]);
+          sc[sl][n][i] = v;
           l_run[n][i & 1] += v;
         }
-#pragma unroll
-      for (int gr = 0; gr < kG; ++gr) {
-        zsum[gr][n][0] *= alpha[n][0];
-        zsum[gr][n][1] *= alpha[n][1];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          acc[gr][i][n][0] *= alpha[n][0];
-          acc[gr][i][n][1] *= alpha[n][1];
-          acc[gr][i][n][2] *= alpha[n][0];
-          acc[gr][i][n][3] *= alpha[n][1];
-        }
-      }
     }
     // output: channels x keys
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      const int ka = mt * 16 + key_a, kb = ka + 8;
+    for (int sl = 0; sl < kSlots; ++sl) {
+      const int k0 = sl * 16 * KP;
+      uint32_t pa[kG], pb[kG];
+      load_params<kG>(vp + (k0 + own) * (D / 8), pa);
+      load_params<kG>(vp + (k0 + own + 8) * (D / 8), pb);
 #pragma unroll
       for (int gr = 0; gr < kG; ++gr) {
-        const uint32_t pa = *reinterpret_cast<const uint32_t*>(vp + ka * (D / 8) + 4 * gr);
-        const uint32_t pb = *reinterpret_cast<const uint32_t*>(vp + kb * (D / 8) + 4 * gr);
-        const float sa = bf16_lo(pa), sb = bf16_lo(pb);
-        const float za = fmaf(8.f, sa, bf16_hi(pa)), zb = fmaf(8.f, sb, bf16_hi(pb));
-        uint32_t a[2][4];
-        const unsigned char* word = vc + (mt * 16 + t) * (D / 2) + 16 * gr + 4 * (g >> 1);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(word + (8 * half) * (D / 2));
-          const uint32_t w1 = *reinterpret_cast<const uint32_t*>(word + (8 * half + 4) * (D / 2));
-          const uint32_t byte = 2 * (g & 1);
-          const uint32_t x0 = __byte_perm(w0, w1, 0x4400 + 0x1111 * byte);
-          const uint32_t x1 = __byte_perm(w0, w1, 0x4400 + 0x1111 * (byte + 1));
-          a[0][2 * half] = codes_bf16(x0);
-          a[0][2 * half + 1] = codes_bf16(x0 >> 4);
-          a[1][2 * half] = codes_bf16(x1);
-          a[1][2 * half + 1] = codes_bf16(x1 >> 4);
-        }
+        const float sa = bf16_lo(pa[gr]), sb = bf16_lo(pb[gr]);
+        const float za = fmaf(8.f, sa, bf16_hi(pa[gr])), zb = fmaf(8.f, sb, bf16_hi(pb[gr]));
+        uint32_t bp[NT][S::kPParts][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float ps[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float v = sc[mt][n][i], sg = i < 2 ? sa : sb, zg = i < 2 ? za : zb;
-            // a masked key's parameters may be anything
-            ps[i] = v > 0.f || v != v ? v * sg : 0.f;
-            zsum[gr][n][i & 1] += v > 0.f || v != v ? v * zg : 0.f;
+            ps[i] = sc[sl][n][i] * (i < 2 ? sa : sb);
+            zsum[gr][n][i & 1] = fmaf(sc[sl][n][i], i < 2 ? za : zb, zsum[gr][n][i & 1]);
           }
 #pragma unroll
           for (int part = 0; part < S::kPParts; ++part) {
             const uint32_t p0 = pack_bf16(ps[0], ps[1]), p1 = pack_bf16(ps[2], ps[3]);
-            const uint32_t b0 = transpose8x8(p0), b1 = transpose8x8(p1);
-            mma_bf16(acc[gr][0][n], a[0], b0, b1);
-            mma_bf16(acc[gr][1][n], a[1], b0, b1);
-            ps[0] -= bf16_lo(p0);
-            ps[1] -= bf16_hi(p0);
-            ps[2] -= bf16_lo(p1);
-            ps[3] -= bf16_hi(p1);
+            bp[n][part][0] = transpose8x8(p0);
+            bp[n][part][1] = transpose8x8(p1);
+            if (part + 1 < S::kPParts) {
+              ps[0] -= bf16_lo(p0);
+              ps[1] -= bf16_hi(p0);
+              ps[2] -= bf16_lo(p1);
+              ps[3] -= bf16_hi(p1);
+            }
           }
+        }
+#pragma unroll
+        for (int k = 0; k < KP; ++k) {
+          uint32_t a[2][4];
+          const unsigned char* word = vc + (k0 + 16 * k + t) * (D / 2) + 16 * gr + 4 * (g >> 1);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(word + (8 * half) * (D / 2));
+            const uint32_t w1 = *reinterpret_cast<const uint32_t*>(word + (8 * half + 4) * (D / 2));
+            const uint32_t x0 = __byte_perm(w0, w1, byte0), x1 = __byte_perm(w0, w1, byte1);
+            a[0][2 * half] = codes_bf16(x0);
+            a[0][2 * half + 1] = codes_bf16(x0 >> 4);
+            a[1][2 * half] = codes_bf16(x1);
+            a[1][2 * half + 1] = codes_bf16(x1 >> 4);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int part = 0; part < S::kPParts; ++part) {
+              const bool mine = KP == 1 || (g >> 2) == k;
+              const uint32_t b0 = mine ? bp[n][part][0] : 0u, b1 = mine ? bp[n][part][1] : 0u;
+              mma_bf16(acc[gr][0][n], a[0], b0, b1);
+              mma_bf16(acc[gr][1][n], a[1], b0, b1);
+            }
         }
       }
     }
@@ -604,39 +709,36 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
   // the four warps' states meet in shared memory; every copy issued has been waited for unless a wait
   // failed, and then the ring is not reused
   __shared__ float w_m[kDecWarps][S::kCols], w_l[kDecWarps][S::kCols];
-  __shared__ int any_failed;
-  if (threadIdx.x == 0) any_failed = 0;
-  __syncthreads();
-  if (failed) any_failed = 1;
+  const bool any_failed = __syncthreads_or(failed);
+  float* w_o = reinterpret_cast<float*>(smem + 128);  // [warp][column][D]
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
+      for (int o = KP == 2 ? 2 : 4; o < 32; o <<= 1) {
         l_run[n][j] += __shfl_xor_sync(0xFFFFFFFFu, l_run[n][j], o);
 #pragma unroll
         for (int gr = 0; gr < kG; ++gr) zsum[gr][n][j] += __shfl_xor_sync(0xFFFFFFFFu, zsum[gr][n][j], o);
       }
-      if (g == 0) {
-        w_m[warp][8 * n + 2 * t + j] = m_run[n][j];
-        w_l[warp][8 * n + 2 * t + j] = l_run[n][j];
+      const int c = (KP == 2 ? 2 * (t & 1) : 8 * n + 2 * t) + j;
+      if (g == 0 && (KP == 1 || t < 2)) {
+        w_m[warp][c] = m_run[n][j];
+        w_l[warp][c] = l_run[n][j];
+      }
+#pragma unroll
+      for (int gr = 0; gr < kG; ++gr) {
+        float o[4] = {acc[gr][0][n][j], acc[gr][0][n][2 + j], acc[gr][1][n][j], acc[gr][1][n][2 + j]};
+        if constexpr (KP == 2) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] += __shfl_xor_sync(0xFFFFFFFFu, o[i], 2);
+        }
+        const float z = zsum[gr][n][j];
+        if (!any_failed && (KP == 1 || t < 2))
+          *reinterpret_cast<float4*>(w_o + (warp * S::kCols + c) * D + kGroup * gr + 4 * g) =
+              make_float4(o[0] + z, o[1] + z, o[2] + z, o[3] + z);
       }
     }
-  __syncthreads();
-  float* w_o = reinterpret_cast<float*>(smem + 128);  // [warp][column][D]
-  if (!any_failed) {
-#pragma unroll
-    for (int gr = 0; gr < kG; ++gr)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float z = zsum[gr][n][j];
-          *reinterpret_cast<float4*>(w_o + (warp * S::kCols + 8 * n + 2 * t + j) * D + kGroup * gr + 4 * g) =
-              make_float4(acc[gr][0][n][j] + z, acc[gr][0][n][2 + j] + z, acc[gr][1][n][j] + z, acc[gr][1][n][2 + j] + z);
-        }
-  }
   __syncthreads();
   const bool last = p.n_chunks == 1;
   const int64_t problem = ((int64_t)b * p.c.n_kv + h) * p.col_tiles + ct;
@@ -673,45 +775,33 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
 }
 
 // Joins the chunks of one (sequence, kv head, column): blockIdx.x < n_cols; the blocks behind add the
-// softmax weights of 1024 keys each.
+// softmax weights of 1024 keys each.  Every warp reads the chunks' maxima and sums for itself.
+constexpr int kJoinThreads = 256;
+
 template <typename T, int D, int COLS>
-__global__ void __launch_bounds__(512) kv4_join_kernel(const Kv4DecParams p) {
+__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Kv4DecParams p) {
   const int h = blockIdx.y, b = blockIdx.z;
   const int64_t len = seq_len_of(p, b);
   const int chunks = max((int)((len + p.chunk_keys - 1) / p.chunk_keys), 1);
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31;
   const int join_blocks = p.n_chunks > 1 ? p.n_cols : 0;
-  __shared__ float red[16];
-  __shared__ float bc;
-  __shared__ float part[512];
+  const int64_t l0 = (int64_t)((int)blockIdx.x - join_blocks) * 1024;
+  if (l0 >= len && (int)blockIdx.x >= join_blocks) return;
+  __shared__ float part[kJoinThreads];
+  pdl_wait();
   auto stats = [&](int col, float* top_out, float* l_out) {  // maximum and sum of a column over its chunks
     const int64_t problem = ((int64_t)b * p.c.n_kv + h) * p.col_tiles + col / COLS;
-    const float* ml = p.part_ml + (problem * p.n_chunks * COLS + col % COLS) * 2;
-    float top = -INFINITY;
-    for (int c = tid; c < chunks; c += 512) top = fmaxf(top, ml[(int64_t)c * COLS * 2]);
-    top = warp_max(top);
-    if ((tid & 31) == 0) red[tid >> 5] = top;
-    __syncthreads();
-    if (tid < 32) {
-      top = warp_max(tid < 16 ? red[tid] : -INFINITY);
-      if (tid == 0) bc = top;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + problem * p.n_chunks * COLS + col % COLS;
+    float top = -INFINITY, l = 0.f;
+    for (int c = lane; c < chunks; c += 32) {
+      const float2 x = ml[(int64_t)c * COLS];
+      const float m_new = fmaxf(top, x.x), use = m_new == -INFINITY ? 0.f : m_new;
+      l = fmaf(l, ex2(top - use), x.y * ex2(x.x - use));
+      top = m_new;
     }
-    __syncthreads();
-    top = bc;
-    const float use = top == -INFINITY ? 0.f : top;
-    float l = 0.f;
-    for (int c = tid; c < chunks; c += 512) l = fmaf(ex2(ml[(int64_t)c * COLS * 2] - use), ml[(int64_t)c * COLS * 2 + 1], l);
-    l = warp_sum(l);
-    if ((tid & 31) == 0) red[tid >> 5] = l;
-    __syncthreads();
-    if (tid < 32) {
-      l = warp_sum(tid < 16 ? red[tid] : 0.f);
-      if (tid == 0) bc = l;
-    }
-    __syncthreads();
-    *top_out = top;
-    *l_out = bc;
-    __syncthreads();
+    const float all = warp_max(top);
+    *l_out = warp_sum(l * ex2(top - (all == -INFINITY ? 0.f : all)));
+    *top_out = all;
   };
   if ((int)blockIdx.x < join_blocks) {
     const int col = blockIdx.x;
@@ -722,15 +812,16 @@ __global__ void __launch_bounds__(512) kv4_join_kernel(const Kv4DecParams p) {
     const int64_t first = problem * p.n_chunks * COLS + col % COLS;
     const int d = tid % D;
     float o = 0.f;
-#pragma unroll 4
-    for (int c = tid / D; c < chunks; c += 512 / D) {
+#pragma unroll 8
+    for (int c = tid / D; c < chunks; c += kJoinThreads / D) {
       const int64_t at = first + (int64_t)c * COLS;
       o = fmaf(ex2(p.part_ml[at * 2] - use), p.part_o[at * D + d], o);
     }
     part[tid] = o;
     __syncthreads();
     if (tid < D) {
-      for (int i = 1; i < 512 / D; ++i) o += part[tid + i * D];
+#pragma unroll
+      for (int i = 1; i < kJoinThreads / D; ++i) o += part[tid + i * D];
       const int tok = col / p.groups, head = h * p.groups + col % p.groups;
       const bool none = top == -INFINITY && l == 0.f;
       reinterpret_cast<T*>(p.out)[b * p.o_seq + (int64_t)head * p.o_head + (int64_t)tok * p.o_row + tid] =
@@ -740,24 +831,26 @@ __global__ void __launch_bounds__(512) kv4_join_kernel(const Kv4DecParams p) {
     }
     return;
   }
-  const int64_t l0 = (int64_t)(blockIdx.x - join_blocks) * 1024;
-  if (l0 >= len) return;
-  float sum[2] = {0.f, 0.f};
+  constexpr int kEach = 1024 / kJoinThreads;
+  float sum[kEach] = {};
   for (int col = 0; col < p.n_cols; ++col) {
+    float x[kEach];
+    const float* row = p.logits + (((int64_t)b * p.c.n_kv + h) * p.n_cols + col) * p.logit_stride;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int64_t key = l0 + j * kJoinThreads + tid;
+      x[j] = key < len ? row[key] : -INFINITY;
+    }
     float top, l;
     stats(col, &top, &l);
     if (top == -INFINITY && l == 0.f) continue;
-    const float* row = p.logits + (((int64_t)b * p.c.n_kv + h) * p.n_cols + col) * p.logit_stride;
     const float inv = 1.f / l;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int64_t key = l0 + j * 512 + tid;
-      if (key < len) sum[j] = fmaf(ex2(row[key] - top), inv, sum[j]);
-    }
+    for (int j = 0; j < kEach; ++j) sum[j] = fmaf(ex2(x[j] - top), inv, sum[j]);
   }
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int64_t key = l0 + j * 512 + tid;
+  for (int j = 0; j < kEach; ++j) {
+    const int64_t key = l0 + j * kJoinThreads + tid;
     if (key < len) p.weights[b * p.w_seq + h * p.w_head + key] += sum[j];
   }
 }
@@ -839,14 +932,15 @@ static int plan_decode(const sva_kv4_cache* c, const sva_kv4_decode_args* a, Kv4
     return set_error(SVA_ERR_SHAPE, "max_len must be within the cache's capacity and below 2^31");
   if (a->dtype < 0 || a->dtype > 2) return set_error(SVA_ERR_DTYPE, "dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
   const int64_t n_cols = (int64_t)(a->n_heads / c->n_kv_heads) * a->n_tokens;
-  // 16 columns a CTA where there are more than 8 (16-bit types): one pass over the cache instead of two
-  plan->cols = (n_cols > 8 && a->dtype != SVA_DTYPE_F32) ? 16 : 8;
+  // 4 columns where they suffice (two key tiles then share an accumulator), 16 where there are more than 8 (one pass
+  // over the cache instead of two); fp32 queries take 8, their three parts fill the registers
+  plan->cols = a->dtype == SVA_DTYPE_F32 ? 8 : (n_cols <= 4 ? 4 : (n_cols <= 8 ? 8 : 16));
   const int64_t tiles = (n_cols + plan->cols - 1) / plan->cols;
   if (n_cols > (1 << 20) || tiles * c->n_kv_heads > 65535) return set_error(SVA_ERR_SHAPE, "too many tokens times heads");
   plan->n_cols = (int)n_cols;
   plan->col_tiles = (int)tiles;
   const int64_t problems = (int64_t)a->n_seqs * c->n_kv_heads * plan->col_tiles;
-  const int64_t slots = 148 * 3;  // CTAs that fit the GPU at once
+  const int64_t slots = 148 * 5;  // CTAs that fit the GPU at once
   const int64_t tiles_k = std::max<int64_t>(1, (a->max_len + kTileKeys - 1) / kTileKeys);
   int64_t chunks = std::max<int64_t>(1, slots / problems);
   // at least 4 tiles a CTA (one a warp); at most 64 where lengths differ, so that long sequences spread
@@ -870,11 +964,11 @@ static int plan_decode(const sva_kv4_cache* c, const sva_kv4_decode_args* a, Kv4
   return SVA_OK;
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int KP>
 static int launch_decode(Kv4DecParams& p, int n_seqs, cudaStream_t st) {
-  using S = DecShape<T, D, NT>;
+  using S = DecShape<T, D, NT, KP>;
   const dim3 grid(p.n_chunks, p.c.n_kv * p.col_tiles, n_seqs);
-  auto* kern = p.weights ? kv4_decode_kernel<T, D, NT, true> : kv4_decode_kernel<T, D, NT, false>;
+  auto* kern = p.weights ? kv4_decode_kernel<T, D, NT, KP, true> : kv4_decode_kernel<T, D, NT, KP, false>;
   int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), S::kSmem);
   if (rc != SVA_OK) return rc;
   kern<<<grid, kDecWarps * 32, S::kSmem, st>>>(p);
@@ -883,16 +977,33 @@ static int launch_decode(Kv4DecParams& p, int n_seqs, cudaStream_t st) {
   const int64_t wblocks = p.weights ? (p.max_len + 1023) / 1024 : 0;
   const int64_t jblocks = (p.n_chunks > 1 ? p.n_cols : 0) + wblocks;
   if (jblocks == 0) return SVA_OK;
-  kv4_join_kernel<T, D, 8 * NT><<<dim3((unsigned)jblocks, p.c.n_kv, n_seqs), 512, 0, st>>>(p);
-  return launched();
+  // launched while the decode kernel drains; it waits there for the decode kernel's memory
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)jblocks, p.c.n_kv, n_seqs);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, D, S::kCols>, p);
+  if (e != cudaSuccess) cudaGetLastError();
+  return e == cudaSuccess ? SVA_OK : set_error(SVA_ERR_CUDA, cudaGetErrorString(e));
+}
+
+template <typename T, int D>
+static int decode_cols(Kv4DecParams& p, int cols, int n_seqs, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (cols == 4) return launch_decode<T, D, 1, 2>(p, n_seqs, st);
+    if (cols == 16) return launch_decode<T, D, 2, 1>(p, n_seqs, st);
+  }
+  return launch_decode<T, D, 1, 1>(p, n_seqs, st);
 }
 
 template <typename T>
 static int decode_dims(Kv4DecParams& p, int D, int cols, int n_seqs, cudaStream_t st) {
-  if constexpr (sizeof(T) == 2) {
-    if (cols == 16) return D == 64 ? launch_decode<T, 64, 2>(p, n_seqs, st) : launch_decode<T, 128, 2>(p, n_seqs, st);
-  }
-  return D == 64 ? launch_decode<T, 64, 1>(p, n_seqs, st) : launch_decode<T, 128, 1>(p, n_seqs, st);
+  return D == 64 ? decode_cols<T, 64>(p, cols, n_seqs, st) : decode_cols<T, 128>(p, cols, n_seqs, st);
 }
 
 }  // namespace sva
