@@ -43,47 +43,156 @@ struct Kv4 {
 // ---------------------------------------------------------------------------------------
 // rows in and out
 // ---------------------------------------------------------------------------------------
-// Eight channels a thread, four threads a group: the group's extremes take two shuffles, a thread's
-// eight codes are one 32-bit word.  HBM bound: D * size + D/2 + D/8 bytes a row.
+// HBM bound: D * size + D/2 + D/8 bytes a row, if a channel takes few instructions.  Writing, a thread has 16 channels (two
+// threads a group: one shuffle joins their extremes, and what is worked out once a group is shared by 16
+// channels); channels go two to an fp32x2 instruction, and numbers become integers by adding 3 * 2^22 (a conversion
+// instruction runs at a quarter of the rate).  Reading, a thread has the 8 channels of one code word.
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, float x[8]) {
-  if constexpr (sizeof(T) == 4) {
-    if (vec) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-      return;
-    }
-  } else {
-    if (vec) {
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-      const T* e = reinterpret_cast<const T*>(&a);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(e[i]);
-      return;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(p[i]);
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
-// Code of x: (x - m) / s to the nearest whole number, halves to even.  For 16-bit inputs the fp32
-// quotient decides: x - m and the halves (k + 1/2) s are fp32 numbers, so a quotient that is a half
-// is found as one.  fp32 inputs leave a remainder in x - m, and the two neighbours are compared in 64 bits.
+constexpr int kWriteChannels = 16;
+
+// A thread's 16 channels as they stand in memory.
 template <typename T>
-__device__ __forceinline__ uint32_t code_of(float x, float m, float s, float inv) {
-  const float d = x - m;
-  float q = d * inv;
-  q = fmaf(fmaf(-q, s, d), inv, q);
-  float c = rintf(q);
-  if constexpr (sizeof(T) == 4) {
-    if (fabsf(fabsf(q - c) - 0.5f) < 1e-4f) {
-      const double base = floor((double)q), rest = ((double)x - (double)m) - (base + 0.5) * (double)s;
-      const bool odd = (((int)base) & 1) != 0;
-      c = (float)((rest > 0.0 || (rest == 0.0 && odd)) ? base + 1.0 : base);
+struct Raw {
+  static constexpr int kVecs = kWriteChannels * sizeof(T) / 16;
+  uint4 v[kVecs];
+};
+
+template <typename T>
+__device__ __forceinline__ void load16(const T* p, bool vec, Raw<T>& r) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < Raw<T>::kVecs; ++i) r.v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    return;
+  }
+  uint32_t* w = reinterpret_cast<uint32_t*>(r.v);
+#pragma unroll
+  for (int i = 0; i < Raw<T>::kVecs * 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      w[i] = __float_as_uint(p[i]);
+    } else {
+      const unsigned short* u = reinterpret_cast<const unsigned short*>(p) + 2 * i;
+      w[i] = u[0] | static_cast<uint32_t>(u[1]) << 16;
     }
   }
-  return (uint32_t)fminf(fmaxf(c, 0.f), 15.f);
+}
+
+// Extremes of the 16 channels; NaN in both where a channel is NaN.
+template <typename T>
+__device__ __forceinline__ void extremes(const Raw<T>& r, float& low, float& high) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(r.v);
+  if constexpr (sizeof(T) == 4) {
+    float odd = 0.f;
+    low = high = __uint_as_float(w[0]);
+#pragma unroll
+    for (int i = 0; i < kWriteChannels; ++i) {
+      const float x = __uint_as_float(w[i]);
+      low = fminf(low, x);
+      high = fmaxf(high, x);
+      odd = fmaf(x, 0.f, odd);  // NaN for a NaN (or an infinity, which is refused all the same)
+    }
+    low += odd;
+    high += odd;
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2* e = reinterpret_cast<const T2*>(r.v);
+    T2 a = e[0], b = e[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+      a = __hmin2_nan(a, e[i]);
+      b = __hmax2_nan(b, e[i]);
+    }
+    low = to_f32<T>(__hmin_nan(a.x, a.y));
+    high = to_f32<T>(__hmax_nan(b.x, b.y));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float element(const Raw<T>& r, int i) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(r.v);
+  if constexpr (sizeof(T) == 4)
+    return __uint_as_float(w[i]);
+  else if constexpr (std::is_same<T, __half>::value)
+    return __half2float(__ushort_as_half((unsigned short)(w[i >> 1] >> (16 * (i & 1)))));
+  else
+    return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+}
+
+// The nearest code where the group's scale is far from the ends of the fp32 range.  The quotient d * inv is corrected by its
+// remainder, so that one that is a half k + 1/2 comes out as exactly that, and adding 3 * 2^22 rounds it to even.  16-bit inputs:
+// the fp32 difference decides.  fp32 inputs: what the difference lost is added to the remainder.
+template <typename T>
+__device__ __forceinline__ uint64_t codes16(const Raw<T>& r, float m, float s) {
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  uint32_t w[2] = {0u, 0u};
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < kWriteChannels; ++i) {
+      const float x = element<T>(r, i), d = x - m, back = d + m;
+      const float lost = (x - back) + (m - (back - d));  // x - m = d + lost
+      const float c = rintf(d * inv);
+      const float rest = fmaf(-c, s, d) + lost, half = 0.5f * s;
+      const bool odd = (static_cast<int>(c) & 1) != 0;
+      const float up = rest > half || (rest == half && odd) ? 1.f : 0.f;
+      const float down = rest < -half || (rest == -half && odd) ? 1.f : 0.f;
+      w[i >> 3] |= static_cast<uint32_t>(static_cast<int>(c + up - down)) << (4 * (i & 7));
+    }
+  } else {
+    const uint64_t m2 = pack2(-m, -m), s2 = pack2(-s, -s), i2 = pack2(inv, inv);
+    const uint64_t round2 = pack2(12582912.f, 12582912.f);
+#pragma unroll
+    for (int i = 0; i < kWriteChannels; i += 2) {
+      const uint64_t d = add2(pack2(element<T>(r, i), element<T>(r, i + 1)), m2);
+      uint64_t q = mul2(d, i2);
+      q = fma2(fma2(q, s2, d), i2, q);
+      q = add2(q, round2);
+      float lo, hi;
+      unpack2(q, lo, hi);
+      // the code is the low bits; each comes in at the top
+      w[i >> 3] = __funnelshift_r(w[i >> 3], __float_as_uint(lo), 4);
+      w[i >> 3] = __funnelshift_r(w[i >> 3], __float_as_uint(hi), 4);
+    }
+  }
+  return static_cast<uint64_t>(w[1]) << 32 | w[0];
+}
+
+// The same in 64 bits, for scales near the ends of the range.
+template <typename T>
+__device__ __forceinline__ uint64_t codes16_wide(const Raw<T>& r, float m, float s) {
+  uint64_t w = 0;
+#pragma unroll 1
+  for (int i = 0; i < kWriteChannels; ++i) {
+    float x = 0.f;
+#pragma unroll
+    for (int j = 0; j < kWriteChannels; ++j) x = j == i ? element<T>(r, j) : x;
+    const double c = rint((static_cast<double>(x) - m) / s);
+    w |= static_cast<uint64_t>(fmin(fmax(c, 0.0), 15.0)) << (4 * i);
+  }
+  return w;
 }
 
 struct Kv4WriteParams {
@@ -97,27 +206,35 @@ struct Kv4WriteParams {
   const int64_t* cu;
 };
 
+constexpr int kWriteRows = 8;   // rows that a thread takes one after another
+constexpr int kWriteAhead = 2;  // of which so many are on their way while one is worked on
+
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4WriteParams p) {
-  constexpr int kLanes = D / 8, kRows = 256 / kLanes, kUnroll = 4;
-  const int which = blockIdx.z;
-  const int h = blockIdx.y % p.c.n_kv, lane = threadIdx.x % kLanes;
-  int b = blockIdx.y / p.c.n_kv;
-  const T* base = reinterpret_cast<const T*>(p.x[which]) + h * p.head_stride[which] + lane * 8;
-  if (!p.cu) base += b * p.seq_stride[which];
-  uint8_t* codes = which ? p.c.v_codes : p.c.k_codes;
-  uint32_t* params = which ? p.c.v_params : p.c.k_params;
-  const int64_t t0 = (int64_t)blockIdx.x * (kRows * kUnroll) + threadIdx.x / kLanes;
-  float x[kUnroll][8];
-  int64_t row[kUnroll];
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const int64_t t = t0 + u * kRows;
-    row[u] = -1;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
-    if (t >= p.n_tokens) continue;
-    int64_t l = t;
+  constexpr int kLanes = D / kWriteChannels, kRows = 256 / kLanes;
+  const bool second = blockIdx.z != 0;
+  const int h = blockIdx.y % p.c.n_kv, lane = threadIdx.x % kLanes, b0 = blockIdx.y / p.c.n_kv;
+  const int64_t row_stride = second ? p.row_stride[1] : p.row_stride[0];
+  const bool vec = second ? p.vec[1] : p.vec[0];
+  const T* base = reinterpret_cast<const T*>(second ? p.x[1] : p.x[0]) + h * (second ? p.head_stride[1] : p.head_stride[0]) +
+                  lane * kWriteChannels;
+  uint64_t* codes = reinterpret_cast<uint64_t*>(second ? p.c.v_codes : p.c.k_codes) + lane;
+  uint32_t* params = (second ? p.c.v_params : p.c.k_params) + (lane >> 1);
+  const int64_t t0 = (int64_t)blockIdx.x * (kRows * kWriteRows) + threadIdx.x / kLanes;
+  int64_t at0 = 0;  // position of token 0
+  if (!p.cu) {
+    base += b0 * (second ? p.seq_stride[1] : p.seq_stride[0]);
+    at0 = __ldg(p.start + b0);
+  }
+  Raw<T> x[kWriteAhead + 1];
+  int64_t row[kWriteAhead + 1];
+  auto fetch = [&](int i, Raw<T>& r, int64_t& to) {
+    const int64_t t = t0 + i * kRows;
+    to = -1;
+    r = Raw<T>{};
+    if (i >= kWriteRows || t >= p.n_tokens) return;
+    int b = b0;
+    int64_t l = at0 + t;
     if (p.cu) {
       // the last sequence that begins at or before t
       int lo = 0, hi = p.n_seqs;
@@ -126,47 +243,43 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4WriteParams p) 
         if (__ldg(p.cu + mid) <= t) lo = mid; else hi = mid;
       }
       b = lo;
-      if (__ldg(p.cu + b) > t || __ldg(p.cu + b + 1) <= t) continue;
-      l = t - __ldg(p.cu + b);
+      if (__ldg(p.cu + b) > t || __ldg(p.cu + b + 1) <= t) return;
+      l = __ldg(p.start + b) + t - __ldg(p.cu + b);
     }
-    row[u] = p.c.row(b, h, __ldg(p.start + b) + l);
-    load8<T>(base + t * p.row_stride[which], p.vec[which], x[u]);
-  }
+    load16<T>(base + t * row_stride, vec, r);
+    to = p.c.row(b, h, l);
+  };
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    float low = x[u][0], high = x[u][0];
-    float sum = 0.f;
+  for (int i = 0; i < kWriteAhead; ++i) fetch(i, x[i], row[i]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      low = fminf(low, x[u][i]);
-      high = fmaxf(high, x[u][i]);
-      sum += x[u][i] * 0.f;  // NaN for a NaN or an infinity
+  for (int i = 0; i < kWriteRows; ++i) {
+    const int now = i % (kWriteAhead + 1), next = (i + kWriteAhead) % (kWriteAhead + 1);
+    fetch(i + kWriteAhead, x[next], row[next]);
+    float low, high;
+    extremes<T>(x[now], low, high);
+    const float low1 = __shfl_xor_sync(0xFFFFFFFFu, low, 1), high1 = __shfl_xor_sync(0xFFFFFFFFu, high, 1);
+    const bool nan = low != low || low1 != low1;
+    low = fminf(low, low1);
+    high = fmaxf(high, high1);
+    // rounded down to bf16: the upper half of the bits, one further from zero below it
+    const uint32_t bits = __float_as_uint(low);
+    const uint32_t mb = (bits + (static_cast<uint32_t>(static_cast<int>(bits) >> 31) & 0xFFFFu)) & 0xFFFF0000u;
+    const float m = __uint_as_float(mb);
+    // (high - m) / 15 rounded up to bf16: a number at or just below it, and the next one if 15 of those fall short
+    const float d = __fsub_ru(high, m);
+    uint32_t sb = (__float_as_uint(d * 0.06666659f) + 0xFFFFu) & 0xFFFF0000u;
+    if (15.f * __uint_as_float(sb) < d) sb += 0x10000u;
+    const float s = __uint_as_float(sb);
+    const bool bad = nan || !(fabsf(m) <= 3.4e38f) || !(s <= 3.4e38f);
+    uint64_t w = 0;
+    if (s > 1e-30f && s < 1e30f) {
+      w = codes16<T>(x[now], m, s);
+    } else if (s > 0.f) {
+      w = codes16_wide<T>(x[now], m, s);
     }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      low = fminf(low, __shfl_xor_sync(0xFFFFFFFFu, low, o));
-      high = fmaxf(high, __shfl_xor_sync(0xFFFFFFFFu, high, o));
-      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    }
-    const __nv_bfloat16 mb = __float2bfloat16_rd(low);
-    const float m = __bfloat162float(mb);
-    const __nv_bfloat16 sb = __float2bfloat16_ru(__fdiv_ru(__fsub_ru(high, m), 15.f));
-    const float s = __bfloat162float(sb);
-    const bool bad = !(sum == 0.f) || !(fabsf(m) <= 3.4e38f) || !(s <= 3.4e38f);
-    // scaling by a power of two keeps 1 / s finite for the smallest scales
-    const float lift = s < 1e-30f ? 0x1p100f : 1.f;
-    const float inv = (s > 0.f && !bad) ? 1.f / (s * lift) : 0.f;
-    uint32_t w = 0;
-    if (!bad) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w |= code_of<T>(x[u][i] * lift, m * lift, s * lift, inv) << (4 * i);
-    }
-    if (row[u] >= 0) {
-      reinterpret_cast<uint32_t*>(codes)[row[u] * kLanes + lane] = w;
-      if ((lane & 3) == 0)
-        params[row[u] * (D / kGroup) + (lane >> 2)] =
-            bad ? 0x7FFF7FFFu
-                : ((uint32_t)__bfloat16_as_ushort(mb) << 16) | (uint32_t)__bfloat16_as_ushort(sb);
+    if (row[now] >= 0) {
+      codes[row[now] * kLanes] = bad ? 0ull : w;
+      if ((lane & 1) == 0) params[row[now] * (D / kGroup)] = bad ? 0x7FFF7FFFu : mb | sb >> 16;
     }
   }
 }
@@ -178,18 +291,20 @@ struct Kv4ReadParams {
   const int64_t* start;
 };
 
+constexpr int kReadUnroll = 4;
+
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
-  constexpr int kLanes = D / 8, kRows = 256 / kLanes, kUnroll = 4;
-  const int which = blockIdx.z;
+  constexpr int kLanes = D / 8, kRows = 256 / kLanes;
+  const bool second = blockIdx.z != 0;
   const int h = blockIdx.y % p.c.n_kv, b = blockIdx.y / p.c.n_kv, lane = threadIdx.x % kLanes;
-  const uint32_t* codes = reinterpret_cast<const uint32_t*>(which ? p.c.v_codes : p.c.k_codes);
-  const uint32_t* params = which ? p.c.v_params : p.c.k_params;
-  const int64_t t0 = (int64_t)blockIdx.x * (kRows * kUnroll) + threadIdx.x / kLanes;
+  const uint32_t* codes = reinterpret_cast<const uint32_t*>(second ? p.c.v_codes : p.c.k_codes);
+  const uint32_t* params = second ? p.c.v_params : p.c.k_params;
+  const int64_t t0 = (int64_t)blockIdx.x * (kRows * kReadUnroll) + threadIdx.x / kLanes;
   const int64_t start = __ldg(p.start + b);
-  uint32_t w[kUnroll], sm[kUnroll];
+  uint32_t w[kReadUnroll], sm[kReadUnroll];
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
+  for (int u = 0; u < kReadUnroll; ++u) {
     const int64_t t = t0 + u * kRows;
     w[u] = sm[u] = 0;
     if (t >= p.n_tokens) continue;
@@ -198,18 +313,37 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
     w[u] = __ldg(codes + row * kLanes + lane);
     sm[u] = __ldg(params + row * (D / kGroup) + (lane >> 2));
   }
-  T* out = reinterpret_cast<T*>(p.out[which]) + (int64_t)blockIdx.y * p.n_tokens * D + lane * 8;
+  T* out = reinterpret_cast<T*>(second ? p.out[1] : p.out[0]) + (int64_t)blockIdx.y * p.n_tokens * D + lane * 8;
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
+  for (int u = 0; u < kReadUnroll; ++u) {
     const int64_t t = t0 + u * kRows;
     if (t >= p.n_tokens) continue;
     const float s = __uint_as_float(sm[u] << 16), m = __uint_as_float(sm[u] & 0xFFFF0000u);
-    __align__(16) T y[8];
+    const uint64_t s2 = pack2(s, s), m2 = pack2(m, m);
+    const uint64_t off = pack2(-128.f, -128.f);
+    float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = from_f32<T>(fmaf(s, (float)((w[u] >> (4 * i)) & 15u), m));
+    for (int i = 0; i < 4; ++i) {
+      // bf16 pair 128 + code, as two fp32 numbers
+      const uint32_t v = ((w[u] >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+      const uint64_t c = add2(pack2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)), off);
+      unpack2(fma2(c, s2, m2), y[i], y[i + 4]);
+    }
     uint4* dst = reinterpret_cast<uint4*>(out + t * D);
-    dst[0] = reinterpret_cast<const uint4*>(y)[0];
-    if constexpr (sizeof(T) == 4) dst[1] = reinterpret_cast<const uint4*>(y)[1];
+    if constexpr (sizeof(T) == 4) {
+      dst[0] = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+      dst[1] = make_uint4(__float_as_uint(y[4]), __float_as_uint(y[5]), __float_as_uint(y[6]), __float_as_uint(y[7]));
+    } else {
+      uint32_t o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __half>::value)
+          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(o[i]) : "f"(y[2 * i + 1]), "f"(y[2 * i]));
+        else
+          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[i]) : "f"(y[2 * i + 1]), "f"(y[2 * i]));
+      }
+      dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
   }
 }
 
@@ -889,7 +1023,7 @@ static int launched() {
 
 template <typename T>
 static int launch_write(const Kv4WriteParams& p, int D, bool packed, cudaStream_t st) {
-  const int64_t rows = 4 * (256 / (D / 8));
+  const int64_t rows = kWriteRows * (256 / (D / kWriteChannels));
   const int64_t blocks = (p.n_tokens + rows - 1) / rows;
   const int64_t ys = (int64_t)p.c.n_kv * (packed ? 1 : p.n_seqs);
   if (blocks > 0x7FFFFFFFll || ys > 65535) return set_error(SVA_ERR_SHAPE, "too many rows, or sequences times kv heads");
@@ -903,7 +1037,7 @@ static int launch_write(const Kv4WriteParams& p, int D, bool packed, cudaStream_
 
 template <typename T>
 static int launch_read(const Kv4ReadParams& p, int D, int n_seqs, cudaStream_t st) {
-  const int64_t rows = 4 * (256 / (D / 8));
+  const int64_t rows = kReadUnroll * (256 / (D / 8));
   const int64_t blocks = (p.n_tokens + rows - 1) / rows;
   const int64_t ys = (int64_t)p.c.n_kv * n_seqs;
   if (blocks > 0x7FFFFFFFll || ys > 65535) return set_error(SVA_ERR_SHAPE, "too many rows, or sequences times kv heads");
