@@ -243,6 +243,13 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
+// The largest of three, one instruction.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   uint32_t r;
@@ -332,6 +339,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
   tc_fence_after();
   const uint32_t tmem = tmem_base;
 
+  // registers from the last four warps to the softmax: 2 x 200 + 96 of the 3 x 168 that the CTA was launched with
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
   if (warp == 8) {
     // ---- copies ----
     if (lane == 0) {
@@ -485,7 +495,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bars.v_clean[st]));
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ---- softmax: a thread owns a row ----
     const int x = warp >> 2, row = (warp & 3) * 32 + lane;
     const int tok = tok0 + x * tp.tokens + row / p.groups;
@@ -493,6 +505,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
     const int limit = live ? limit_of(tok) : 0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + 128 * x + lanes, to = tmem + 256 + DP * x + lanes;
+    const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = first; j < stop[x]; ++j) {
@@ -517,8 +530,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
 #pragma unroll
       for (int i = 0; i < 4; ++i) top[i] = f[i];
 #pragma unroll
-      for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], f[i]);
-      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
+      for (int i = 4; i < 124; i += 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top[k] = max3(top[k], f[i + 2 * k], f[i + 2 * k + 1]);
+      top[0] = max3(top[0], f[124], f[125]);
+      top[1] = max3(top[1], f[126], f[127]);
+      const float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]) * p.scale_log2;
       const bool grew = mx > m + 8.f;
       if (__any_sync(0xFFFFFFFFu, grew)) {
         const float m_new = grew ? mx : m;
@@ -539,21 +556,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
         }
       }
       const float use = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t minus2 = pack2(-use, -use);
+      uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t w[32];
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float e0 = ex2(fmaf(f[64 * c + 2 * i], p.scale_log2, -use));
-          const float e1 = ex2(fmaf(f[64 * c + 2 * i + 1], p.scale_log2, -use));
-          sum[2 * (i & 1)] += e0;
-          sum[2 * (i & 1) + 1] += e1;
+        for (int i = 0; i < 16; ++i) {
+          float e0, e1;
+          unpack2(fma2(pack2(f[32 * c + 2 * i], f[32 * c + 2 * i + 1]), scale2, minus2), e0, e1);
+          e0 = ex2(e0);
+          e1 = ex2(e1);
+          sum[i & 1] = add2(sum[i & 1], pack2(e0, e1));
           w[i] = pack16<T>(e0, e1);
         }
-        tc_st32(ts + 32 * c, w);
+        tc_st16(ts + 16 * c, w);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      float s0, s1;
+      unpack2(add2(sum[0], sum[1]), s0, s1);
+      l += s0 + s1;
       tc_wait_st();
       tc_fence_before();
       mbar_arrive(smem_u32(&bars.p_full[x]));
