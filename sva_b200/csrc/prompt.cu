@@ -220,10 +220,17 @@ struct TcShape {
   static constexpr int kTileBytes = kTcRows * 128 * kHalves;    // one Q, K or V tile
   static constexpr int kStages = DP == 64 ? 3 : 2;
   static constexpr int kSmem = 1024 + kTileBytes * (2 + 2 * kStages);
+  // Tensor memory (512 columns): S of A and B, O of A and B.  With 64 channels there is room for P beside S: the next
+  // block's S is then worked out while this block is in its softmax, and no warp waits for the tensor cores.  With 128, P
+  // takes the place of S.
+  static constexpr bool kApart = DP == 64;
+  __host__ __device__ static constexpr uint32_t s_col(int x) { return 128u * x; }
+  __host__ __device__ static constexpr uint32_t o_col(int x) { return 256u + DP * x; }
+  __host__ __device__ static constexpr uint32_t p_col(int x) { return kApart ? 384u + 64u * x : 128u * x; }
 };
 
 struct TcBars {
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full[2], s_full[2], s_read[2], p_full[2], pv_done[2];
   uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3], v_go[3], v_clean[3];
 };
 
@@ -312,8 +319,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
     for (int x = 0; x < 2; ++x) {
       mbar_init(smem_u32(&bars.q_full[x]), 1);
       mbar_init(smem_u32(&bars.s_full[x]), 1);
+      mbar_init(smem_u32(&bars.s_read[x]), 128);
       mbar_init(smem_u32(&bars.p_full[x]), 128);
-      mbar_init(smem_u32(&bars.o_full[x]), 1);
+      mbar_init(smem_u32(&bars.pv_done[x]), 1);
     }
 #pragma unroll
     for (int i = 0; i < S::kStages; ++i) {
@@ -388,7 +396,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
     }
   } else if (warp == 9) {
     // ---- MMAs ----
-    if (lane == 0) {
+    {
+      // a warp-wide maximum is what the compiler knows to be uniform
+      auto uniform = [](int v) { return __reduce_max_sync(0xFFFFFFFFu, v); };
+      const uint32_t one = elect_one(), tm = (uint32_t)uniform((int)tmem);
+      const int count = uniform(end - first), dirty = uniform(max(0, masked - first));
+      const int counts[2] = {uniform(stop[0] - first), uniform(stop[1] - first)};
+      auto wait = [&](const uint64_t& bar, int turn) { return __all_sync(0xFFFFFFFFu, mbar_wait_or(smem_u32(&bar), turn & 1, failed)) != 0; };
       constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
       constexpr uint32_t kIdescS = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((kTcRows / 8) << 17) | ((kTcRows / 16) << 24);
       constexpr uint32_t kIdescO =
@@ -397,55 +411,69 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
           const uint32_t off = (kk / 4) * kTcRows * 128 + (kk % 4) * 32;
-          tc_mma_ss(tmem + 128 * x, tc_desc(smem_u32(sq + x * S::kTileBytes) + off, 16),
-                    tc_desc(smem_u32(sk + st * S::kTileBytes) + off, 16), kIdescS, kk > 0);
+          tc_mma_ss(tm + S::s_col(x), tc_desc(smem_u32(sq + x * S::kTileBytes) + off, 16),
+                    tc_desc(smem_u32(sk + st * S::kTileBytes) + off, 16), kIdescS, kk > 0, one);
         }
-        tc_commit(smem_u32(&bars.s_full[x]));
+        tc_commit(smem_u32(&bars.s_full[x]), one);
       };
       bool ok = true;
-      if (end > first) ok = mbar_wait_or(smem_u32(&bars.k_full[0]), 0, failed);
+      if (count > 0) ok = wait(bars.k_full[0], 0);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        if (!ok || stop[x] <= first) continue;
-        ok = mbar_wait_or(smem_u32(&bars.q_full[x]), 0, failed);
+        if (!ok || counts[x] <= 0) continue;
+        ok = wait(bars.q_full[x], 0);
         if (ok) scores(x, 0);
       }
-      if (ok && end > first) tc_commit(smem_u32(&bars.k_empty[0]));
-      for (int j = first; j < end && ok; ++j) {
-        const int n = j - first, st = n % S::kStages, turn = n / S::kStages;
+      if (ok && count > 0) tc_commit(smem_u32(&bars.k_empty[0]), one);
+      for (int n = 0; n < count && ok; ++n) {
+        const int st = n % S::kStages, turn = n / S::kStages;
         const int n1 = n + 1, st1 = n1 % S::kStages, turn1 = n1 / S::kStages;
         bool k_ready = false;
-        ok = mbar_wait_or(smem_u32(&bars.v_full[st]), turn & 1, failed);
+        auto next_scores = [&](int x) {
+          if (!ok || n + 1 >= counts[x]) return;
+          if (!k_ready) ok = wait(bars.k_full[st1], turn1);
+          k_ready = true;
+          if (ok) scores(x, st1);
+        };
+        if constexpr (S::kApart) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (!ok || n + 1 >= counts[x]) continue;
+            ok = wait(bars.s_read[x], n);
+            tc_fence_after();
+            next_scores(x);
+          }
+          if (ok && n + 1 < count) tc_commit(smem_u32(&bars.k_empty[st1]), one);
+        }
+        if (ok) ok = wait(bars.v_full[st], turn);
         // blocks with keys that some row may not see: wait for their value rows to be cleaned
-        if (ok && j >= masked) ok = mbar_wait_or(smem_u32(&bars.v_clean[st]), clean_turn(j) & 1, failed);
+        if (ok && n >= dirty) ok = wait(bars.v_clean[st], (n - dirty) / S::kStages);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          if (!ok || j >= stop[x]) continue;
-          ok = mbar_wait_or(smem_u32(&bars.p_full[x]), n & 1, failed);
+          if (!ok || n >= counts[x]) continue;
+          ok = wait(bars.p_full[x], n);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < kTcRows / 16; ++kk)
-            tc_mma_ts(tmem + 256 + DP * x, tmem + 128 * x + 8 * kk,
-                      tc_desc(smem_u32(sv + st * S::kTileBytes) + kk * 2048, kTcRows * 128), kIdescO, n > 0 || kk > 0);
-          if (j + 1 < stop[x]) {
-            if (!k_ready) ok = mbar_wait_or(smem_u32(&bars.k_full[st1]), turn1 & 1, failed);
-            k_ready = true;
-            if (ok) scores(x, st1);
-          } else {
-            tc_commit(smem_u32(&bars.o_full[x]));
-          }
+            tc_mma_ts(tm + S::o_col(x), tm + S::p_col(x) + 8 * kk,
+                      tc_desc(smem_u32(sv + st * S::kTileBytes) + kk * 2048, kTcRows * 128), kIdescO, n > 0 || kk > 0, one);
+          if (S::kApart || n + 1 >= counts[x]) tc_commit(smem_u32(&bars.pv_done[x]), one);
+          if constexpr (!S::kApart) next_scores(x);
         }
         if (!ok) break;
-        tc_commit(smem_u32(&bars.v_empty[st]));
-        if (j + 1 < end) tc_commit(smem_u32(&bars.k_empty[st1]));
+        tc_commit(smem_u32(&bars.v_empty[st]), one);
+        if (!S::kApart && n + 1 < count) tc_commit(smem_u32(&bars.k_empty[st1]), one);
       }
       if (!ok) {
         // the MMAs issued so far end before the tensor memory is released
         __shared__ uint64_t drain;
-        mbar_init(smem_u32(&drain), 1);
-        mbar_fence_init();
-        tc_commit(smem_u32(&drain));
+        if (lane == 0) {
+          mbar_init(smem_u32(&drain), 1);
+          mbar_fence_init();
+        }
+        __syncwarp();
+        tc_commit(smem_u32(&drain), one);
         mbar_wait(smem_u32(&drain), 0);
       }
     }
@@ -504,7 +532,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
     const bool live = row < tp.tokens * p.groups && tok < s.len_q;
     const int limit = live ? limit_of(tok) : 0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + 128 * x + lanes, to = tmem + 256 + DP * x + lanes;
+    const uint32_t ts = tmem + S::s_col(x) + lanes, to = tmem + S::o_col(x) + lanes, tpr = tmem + S::p_col(x) + lanes;
     const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
@@ -520,6 +548,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
       for (int c = 0; c < 4; ++c) tc_ld32(ts + 32 * c, v + 32 * c);
       tc_wait_ld();
       tc_pin<128>(v);
+      if constexpr (S::kApart) {
+        tc_fence_before();
+        mbar_arrive(smem_u32(&bars.s_read[x]));
+      }
       float* f = reinterpret_cast<float*>(v);
       if (j >= masked) {
         const int seen = limit - j * kTcRows;
@@ -537,12 +569,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
       top[1] = max3(top[1], f[126], f[127]);
       const float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]) * p.scale_log2;
       const bool grew = mx > m + 8.f;
+      // O and P are free once the block before has been added.  (P in the place of S: that S is complete says so.)
+      if (S::kApart && n > 0) {
+        if (!mbar_wait_or(smem_u32(&bars.pv_done[x]), (n - 1) & 1, failed)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+      }
       if (__any_sync(0xFFFFFFFFu, grew)) {
         const float m_new = grew ? mx : m;
         const float alpha = grew ? ex2(m - m_new) : 1.f;  // 0 from -inf
         m = m_new;
         l *= alpha;
-        if (n > 0) {  // S of this block is complete, so O is complete up to the block before
+        if (n > 0) {
 #pragma unroll
           for (int c = 0; c < DP / 32; ++c) {
             uint32_t o[32];
@@ -570,7 +610,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
           sum[i & 1] = add2(sum[i & 1], pack2(e0, e1));
           w[i] = pack16<T>(e0, e1);
         }
-        tc_st16(ts + 16 * c, w);
+        tc_st16(tpr + 16 * c, w);
       }
       float s0, s1;
       unpack2(add2(sum[0], sum[1]), s0, s1);
@@ -580,7 +620,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
       mbar_arrive(smem_u32(&bars.p_full[x]));
     }
     const bool any = stop[x] > first;
-    if (ok && any) ok = mbar_wait_or(smem_u32(&bars.o_full[x]), 0, failed);
+    if (ok && any) ok = mbar_wait_or(smem_u32(&bars.pv_done[x]), S::kApart ? (stop[x] - first - 1) & 1 : 0, failed);
     tc_fence_after();
     const int head = h * p.groups + row % p.groups;
     const int64_t qrow = s.q0 + tok;
