@@ -427,23 +427,31 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return r;
 }
 
+// Two codes around 8 in fp16 from the low (high) halves of both halves of v: 0x6400 is 1024 with the code in its lowest (16 times
+// the code in its next) mantissa bits; 1032, 1/16 and -72.
+__device__ __forceinline__ uint32_t codes_f16_lo(uint32_t v) {
+  const uint32_t x = (v & 0x000F000Fu) | 0x64006400u;
+  const __half2 d = __hsub2(reinterpret_cast<const __half2&>(x), __half2half2(__ushort_as_half(0x6408)));
+  return reinterpret_cast<const uint32_t&>(d);
+}
+__device__ __forceinline__ uint32_t codes_f16_hi(uint32_t v) {
+  const uint32_t x = (v & 0x00F000F0u) | 0x64006400u;
+  const __half2 d = __hfma2(reinterpret_cast<const __half2&>(x), __half2half2(__ushort_as_half(0x2C00)),
+                            __half2half2(__ushort_as_half(0xD480)));
+  return reinterpret_cast<const uint32_t&>(d);
+}
+
 // A word's eight codes around 8 as the pairs (i, i + 4), i = 0..3, of a score operand: in fp16 for 16-bit queries, where two of
-// the four pairs need no shift (9 instructions a word), in bf16 for fp32 queries, whose three bf16 parts keep every bit.
-template <bool kHalf>
+// the four pairs need no shift (9 instructions a word), in bf16 for fp32 queries, whose three bf16 parts keep every bit.  (Read
+// as e4m3 bytes the codes would be exact as they stand, 2^-9 times the code, but mma.sync on bytes compiles to conversions here:
+// 224 registers instead of 99.)
+template <bool kWide>
 __device__ __forceinline__ void code_fragments(uint32_t w, uint32_t r[4]) {
-  if constexpr (kHalf) {
-    // 0x6400 is 1024: 1024 + c from the low nibbles, 1024 + 16 c from the high ones
-    const uint32_t u = w >> 8;
-    const uint32_t x[4] = {(w & 0x000F000Fu) | 0x64006400u, (w & 0x00F000F0u) | 0x64006400u,
-                           (u & 0x000F000Fu) | 0x64006400u, (u & 0x00F000F0u) | 0x64006400u};
-    const __half2 k1032 = __half2half2(__ushort_as_half(0x6408)), k16 = __half2half2(__ushort_as_half(0x2C00)),
-                  k72 = __half2half2(__ushort_as_half(0xD480));  // 1032, 1/16, -72
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __half2 h = reinterpret_cast<const __half2&>(x[i]);
-      const __half2 d = i & 1 ? __hfma2(h, k16, k72) : __hsub2(h, k1032);
-      r[i] = reinterpret_cast<const uint32_t&>(d);
-    }
+  if constexpr (!kWide) {
+    r[0] = codes_f16_lo(w);
+    r[1] = codes_f16_hi(w);
+    r[2] = codes_f16_lo(w >> 8);
+    r[3] = codes_f16_hi(w >> 8);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) r[i] = codes_bf16(w >> (4 * i));
@@ -455,8 +463,7 @@ __device__ __forceinline__ void code_fragments(uint32_t w, uint32_t r[4]) {
 template <typename T, int D, int NT, int KP>
 struct DecShape {
   static constexpr bool kWide = sizeof(T) == 4;
-  static constexpr int kQParts = kWide ? 3 : 1;                                          // bf16 parts of q
-  static constexpr int kPParts = kWide ? 3 : (std::is_same<T, __half>::value ? 2 : 1);  // and of p s
+  static constexpr int kParts = kWide ? 3 : 1;  // operands that q, and p s, are split into: bf16, or one of fp16
   static constexpr int kGroups = D / kGroup;
   static constexpr int kTileBytes = kTileKeys * (D / 2 + D / 8) * 2;
   static constexpr int kStages = 2;
@@ -480,7 +487,6 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
   using S = DecShape<T, D, NT, KP>;
   static_assert(KP == 1 || NT == 1, "shared accumulators hold one column tile");
   constexpr int kG = S::kGroups, kStages = S::kStages, kSlots = 4 / KP;
-  constexpr bool kHalf = !S::kWide;
   extern __shared__ __align__(128) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int ct = blockIdx.y % p.col_tiles, h = blockIdx.y / p.col_tiles, b = blockIdx.z;
@@ -530,10 +536,8 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
   for (int s = 0; s < kStages; ++s)
     if (s < my_tiles) issue(s, 0);
 
-  // query fragments: the lane's column (g, or g % 4), channels 32 G + 8 t .. + 7, pairs (i, i + 4).  16-bit queries are
-  // scaled by a power of two that brings a column's largest element into [1, 2): exact in fp16, but for what lies
-  // 2^-14 below the largest, which is off by at most 2^-25 of it.
-  uint32_t qf[kG][S::kQParts][KP][NT][4];
+  // query fragments: the lane's column (g, or g % 4), channels 32 G + 8 t .. + 7
+  uint32_t qf[kG][S::kParts][KP][NT][4];
   float qsum[kG][NT][2], scale[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -547,23 +551,27 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         x[gr][i] = live ? to_f32<T>(src[gr * kGroup + 8 * t + i]) : 0.f;
+        if (p.scale_log2 < 0.f) x[gr][i] = -x[gr][i];  // the scale below is then positive
         big = fmaxf(big, fabsf(x[gr][i]));
       }
-    if constexpr (kHalf) {
+    if constexpr (!S::kWide) {
       big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
+      // the power of two that brings the column's largest element to [1, 2): exact in fp16, but for what lies 2^-14 below the
+      // largest, which is off by at most 2^-25 of it
       const uint32_t e = min(max(__float_as_uint(big) >> 23, 1u), 253u);
+      const float factor = __uint_as_float((254u - e) << 23);
       unit = __uint_as_float(e << 23);
-      const float down = __uint_as_float((254u - e) << 23);
 #pragma unroll
       for (int gr = 0; gr < kG; ++gr)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[gr][i] *= down;
+        for (int i = 0; i < 8; ++i) x[gr][i] *= factor;
     }
-    // this lane accumulates columns 2t and 2t + 1 (mod 4)
+    // this lane accumulates columns 2t and 2t + 1 (mod 4).  A scale of 0 would make NaN of a masked -inf.
     const int c = KP == 2 ? 2 * (t & 1) : 2 * t;
-    scale[n][0] = p.scale_log2 * __shfl_sync(0xFFFFFFFFu, unit, c * 4);
-    scale[n][1] = p.scale_log2 * __shfl_sync(0xFFFFFFFFu, unit, (c + 1) * 4);
+    const float to_log2 = fmaxf(fabsf(p.scale_log2), 1e-37f);
+    scale[n][0] = to_log2 * __shfl_sync(0xFFFFFFFFu, unit, c * 4);
+    scale[n][1] = to_log2 * __shfl_sync(0xFFFFFFFFu, unit, (c + 1) * 4);
 #pragma unroll
     for (int gr = 0; gr < kG; ++gr) {
       float sum = 0.f;
@@ -574,17 +582,18 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
       qsum[gr][n][0] = __shfl_sync(0xFFFFFFFFu, sum, c * 4);
       qsum[gr][n][1] = __shfl_sync(0xFFFFFFFFu, sum, (c + 1) * 4);
 #pragma unroll
-      for (int part = 0; part < S::kQParts; ++part) {
+      for (int part = 0; part < S::kParts; ++part) {
+        uint32_t v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t v = kHalf ? pack_f16(x[gr][i], x[gr][i + 4]) : pack_bf16(x[gr][i], x[gr][i + 4]);
-#pragma unroll
-          for (int k = 0; k < KP; ++k) qf[gr][part][k][n][i] = KP == 1 || (g >> 2) == k ? v : 0u;
-          if constexpr (S::kQParts > 1) {
-            x[gr][i] -= bf16_lo(v);
-            x[gr][i + 4] -= bf16_hi(v);
-          }
+          v[i] = S::kWide ? pack_bf16(x[gr][i], x[gr][i + 4]) : pack_f16(x[gr][i], x[gr][i + 4]);
+          x[gr][i] -= bf16_lo(v[i]);
+          x[gr][i + 4] -= bf16_hi(v[i]);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int k = 0; k < KP; ++k) qf[gr][part][k][n][i] = KP == 1 || (g >> 2) == k ? v[i] : 0u;
       }
     }
   }
@@ -601,7 +610,11 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
   const int seen_all = (int)min(max(len - p.n_tokens + 1 - key0, (int64_t)0), p.chunk_keys);
   const int seen_any = (int)(key1 - key0);
 
+  // m_run: the largest scaled score so far; weights are taken relative to m_run + lift.  fp16 weights times scales: lift is the
+  // exponent above the largest scale of V so far (the same for the warp's columns), so that no product passes 1.
   float m_run[NT][2], l_run[NT][2], zsum[kG][NT][2], acc[kG][2][NT][4];
+  float lift = 0.f;
+  uint32_t scale_bound = 0;  // bf16 bits of 2^lift
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -670,20 +683,20 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
         for (int k = 0; k < KP; ++k) {
           const unsigned char* word = kc + (k0 + 16 * k + key_a) * (D / 2) + 16 * gr + 4 * t;
           uint32_t fa[4], fb[4];
-          code_fragments<kHalf>(*reinterpret_cast<const uint32_t*>(word), fa);
-          code_fragments<kHalf>(*reinterpret_cast<const uint32_t*>(word + 8 * (D / 2)), fb);
-          const uint32_t a0[4] = {fa[0], fb[0], fa[1], fb[1]}, a1[4] = {fa[2], fb[2], fa[3], fb[3]};
+          code_fragments<S::kWide>(*reinterpret_cast<const uint32_t*>(word), fa);
+          code_fragments<S::kWide>(*reinterpret_cast<const uint32_t*>(word + 8 * (D / 2)), fb);
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int part = 0; part < S::kQParts; ++part) {
+            for (int part = 0; part < S::kParts; ++part) {
               const uint32_t* q = qf[gr][part][k][n];
-              if constexpr (kHalf) {
-                mma_f16(c[n], a0, q[0], q[1]);
-                mma_f16(c[n], a1, q[2], q[3]);
-              } else {
+              const uint32_t a0[4] = {fa[0], fb[0], fa[1], fb[1]}, a1[4] = {fa[2], fb[2], fa[3], fb[3]};
+              if constexpr (S::kWide) {
                 mma_bf16(c[n], a0, q[0], q[1]);
                 mma_bf16(c[n], a1, q[2], q[3]);
+              } else {
+                mma_f16(c[n], a0, q[0], q[1]);
+                mma_f16(c[n], a1, q[2], q[3]);
               }
             }
         }
@@ -696,7 +709,29 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
             sc[sl][n][i] = fmaf(i < 2 ? sa : sb, c[n][i], fmaf(i < 2 ? za : zb, qsum[gr][n][i & 1], sc[sl][n][i]));
       }
     }
-    // scale, mask, running maximum
+    // a scale of V above the bound?  (NaN groups do not count: they make their own channels NaN)
+    bool lifted = false;
+    if constexpr (!S::kWide) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int i = 0; i < kG / 2; ++i) {
+        const uint4 w = *reinterpret_cast<const uint4*>(vp + 16 * (lane + 32 * i));
+        most = max(most, max(max(w.x & 0xFFFFu, w.y & 0xFFFFu), max(w.z & 0xFFFFu, w.w & 0xFFFFu)));
+      }
+      if (__any_sync(0xFFFFFFFFu, most > scale_bound)) {
+        most = 0;
+        for (int e = lane; e < kTileKeys * kG; e += 32) {
+          const uint32_t w = reinterpret_cast<const uint32_t*>(vp)[e] & 0xFFFFu;
+          most = max(most, w < 0x7F80u ? w : 0u);
+        }
+        most = __reduce_max_sync(0xFFFFFFFFu, most);
+        if (most > scale_bound) {
+          scale_bound = min(max((most >> 7) + 1, 27u), 227u) << 7;
+          lifted = true;
+        }
+      }
+    }
+    // mask, running maximum
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float top[2] = {-INFINITY, -INFINITY};
@@ -704,30 +739,33 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
       for (int sl = 0; sl < kSlots; ++sl)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float v = sc[sl][n][i] * scale[n][i & 1];
           const int l = l0 + sl * 16 * KP + own + (i < 2 ? 0 : 8);
-          if (!whole) v = there && l < limit[n][i & 1] ? v : -INFINITY;
-          sc[sl][n][i] = v;
-          top[i & 1] = fmaxf(top[i & 1], v);
+          if (!whole) sc[sl][n][i] = there && l < limit[n][i & 1] ? sc[sl][n][i] : -INFINITY;
+          top[i & 1] = fmaxf(top[i & 1], sc[sl][n][i]);
           if constexpr (kLogits) {
             const int col = col0 + (KP == 2 ? 2 * (t & 1) : 8 * n + 2 * t) + (i & 1);
             if (col < p.n_cols && l < seen_any)
-              p.logits[(((int64_t)b * p.c.n_kv + h) * p.n_cols + col) * p.logit_stride + key0 + l] = v;
+              p.logits[(((int64_t)b * p.c.n_kv + h) * p.n_cols + col) * p.logit_stride + key0 + l] =
+                  sc[sl][n][i] * scale[n][i & 1];
           }
         }
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int o = KP == 2 ? 2 : 4; o < 32; o <<= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xFFFFFFFFu, top[j], o));
-      if (__any_sync(0xFFFFFFFFu, top[0] > m_run[n][0] || top[1] > m_run[n][1])) {
+        top[j] *= scale[n][j];
+      }
+      if (__any_sync(0xFFFFFFFFu, lifted || top[0] > m_run[n][0] || top[1] > m_run[n][1])) {
+        const float now = S::kWide ? 0.f : static_cast<float>(static_cast<int>(scale_bound >> 7) - 127);
         float alpha[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const float m_new = fmaxf(m_run[n][j], top[j]);
-          alpha[j] = m_new == -INFINITY ? 0.f : ex2(m_run[n][j] - m_new);
+          alpha[j] = m_new == -INFINITY ? 0.f : ex2((m_run[n][j] - m_new) + (lift - now));
           m_run[n][j] = m_new;
           l_run[n][j] *= alpha[j];
         }
+        if (n == NT - 1) lift = now;
 #pragma unroll
         for (int gr = 0; gr < kG; ++gr) {
           zsum[gr][n][0] *= alpha[0];
@@ -736,12 +774,15 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
           for (int i = 0; i < 8; ++i) acc[gr][i >> 2][n][i & 3] *= alpha[i & 1];
         }
       }
-      const float use[2] = {m_run[n][0] == -INFINITY ? 0.f : m_run[n][0], m_run[n][1] == -INFINITY ? 0.f : m_run[n][1]};
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float use[2] = {m_run[n][0] == -INFINITY ? 0.f : m_run[n][0] + lift, m_run[n][1] == -INFINITY ? 0.f : m_run[n][1] + lift};
 #pragma unroll
       for (int sl = 0; sl < kSlots; ++sl)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float v = ex2(sc[sl][n][i] - use[i & 1]);
+          const float v = ex2(fmaf(sc[sl][n][i], scale[n][i & 1], -use[i & 1]));
           sc[sl][n][i] = v;
           l_run[n][i & 1] += v;
         }
@@ -757,7 +798,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
       for (int gr = 0; gr < kG; ++gr) {
         const float sa = bf16_lo(pa[gr]), sb = bf16_lo(pb[gr]);
         const float za = fmaf(8.f, sa, bf16_hi(pa[gr])), zb = fmaf(8.f, sb, bf16_hi(pb[gr]));
-        uint32_t bp[NT][S::kPParts][2];
+        uint32_t bp[NT][S::kParts][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float ps[4];
@@ -767,11 +808,12 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
             zsum[gr][n][i & 1] = fmaf(sc[sl][n][i], i < 2 ? za : zb, zsum[gr][n][i & 1]);
           }
 #pragma unroll
-          for (int part = 0; part < S::kPParts; ++part) {
-            const uint32_t p0 = pack_bf16(ps[0], ps[1]), p1 = pack_bf16(ps[2], ps[3]);
+          for (int part = 0; part < S::kParts; ++part) {
+            const uint32_t p0 = S::kWide ? pack_bf16(ps[0], ps[1]) : pack_f16(ps[0], ps[1]);
+            const uint32_t p1 = S::kWide ? pack_bf16(ps[2], ps[3]) : pack_f16(ps[2], ps[3]);
             bp[n][part][0] = transpose8x8(p0);
             bp[n][part][1] = transpose8x8(p1);
-            if (part + 1 < S::kPParts) {
+            if (part + 1 < S::kParts) {
               ps[0] -= bf16_lo(p0);
               ps[1] -= bf16_hi(p0);
               ps[2] -= bf16_lo(p1);
@@ -788,19 +830,24 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
             const uint32_t w0 = *reinterpret_cast<const uint32_t*>(word + (8 * half) * (D / 2));
             const uint32_t w1 = *reinterpret_cast<const uint32_t*>(word + (8 * half + 4) * (D / 2));
             const uint32_t x0 = __byte_perm(w0, w1, byte0), x1 = __byte_perm(w0, w1, byte1);
-            a[0][2 * half] = codes_bf16(x0);
-            a[0][2 * half + 1] = codes_bf16(x0 >> 4);
-            a[1][2 * half] = codes_bf16(x1);
-            a[1][2 * half + 1] = codes_bf16(x1 >> 4);
+            a[0][2 * half] = S::kWide ? codes_bf16(x0) : codes_f16_lo(x0);
+            a[0][2 * half + 1] = S::kWide ? codes_bf16(x0 >> 4) : codes_f16_hi(x0);
+            a[1][2 * half] = S::kWide ? codes_bf16(x1) : codes_f16_lo(x1);
+            a[1][2 * half + 1] = S::kWide ? codes_bf16(x1 >> 4) : codes_f16_hi(x1);
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int part = 0; part < S::kPParts; ++part) {
+            for (int part = 0; part < S::kParts; ++part) {
               const bool mine = KP == 1 || (g >> 2) == k;
               const uint32_t b0 = mine ? bp[n][part][0] : 0u, b1 = mine ? bp[n][part][1] : 0u;
-              mma_bf16(acc[gr][0][n], a[0], b0, b1);
-              mma_bf16(acc[gr][1][n], a[1], b0, b1);
+              if constexpr (S::kWide) {
+                mma_bf16(acc[gr][0][n], a[0], b0, b1);
+                mma_bf16(acc[gr][1][n], a[1], b0, b1);
+              } else {
+                mma_f16(acc[gr][0][n], a[0], b0, b1);
+                mma_f16(acc[gr][1][n], a[1], b0, b1);
+              }
             }
         }
       }
@@ -833,7 +880,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
       }
       const int c = (KP == 2 ? 2 * (t & 1) : 8 * n + 2 * t) + j;
       if (g == 0 && (KP == 1 || t < 2)) {
-        w_m[warp][c] = m_run[n][j];
+        w_m[warp][c] = m_run[n][j] + lift;
         w_l[warp][c] = l_run[n][j];
       }
 #pragma unroll
