@@ -267,6 +267,13 @@ struct Kv4ReadParams {
   const int64_t* start;
 };
 
+// (a & b) | c in one instruction (the compiler takes two where b and c are constants).
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+
 constexpr int kReadUnroll = 4;
 
 template <typename T, int D>
@@ -301,7 +308,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       // bf16 pair 128 + code, as two fp32 numbers
-      const uint32_t v = ((w[u] >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+      const uint32_t v = and_or(w[u] >> (4 * i), 0x000F000Fu, 0x43004300u);
       const uint64_t c = add2(pack2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)), off);
       unpack2(fma2(c, s2, m2), y[i], y[i + 4]);
     }
@@ -407,7 +414,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 // Two codes in the low bits of both halves of v -> bf16 pair of code - 8: 0x4300 is 128 with the code
 // as its lowest mantissa bits, 0x4308 is 136.
 __device__ __forceinline__ uint32_t codes_bf16(uint32_t v) {
-  const uint32_t x = (v & 0x000F000Fu) | 0x43004300u;
+  const uint32_t x = and_or(v, 0x000F000Fu, 0x43004300u);
   const __nv_bfloat162 d = __hsub2(reinterpret_cast<const __nv_bfloat162&>(x),
                                    __nv_bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308)));
   return reinterpret_cast<const uint32_t&>(d);
@@ -430,12 +437,12 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 // Two codes around 8 in fp16 from the low (high) halves of both halves of v: 0x6400 is 1024 with the code in its lowest (16 times
 // the code in its next) mantissa bits; 1032, 1/16 and -72.
 __device__ __forceinline__ uint32_t codes_f16_lo(uint32_t v) {
-  const uint32_t x = (v & 0x000F000Fu) | 0x64006400u;
+  const uint32_t x = and_or(v, 0x000F000Fu, 0x64006400u);
   const __half2 d = __hsub2(reinterpret_cast<const __half2&>(x), __half2half2(__ushort_as_half(0x6408)));
   return reinterpret_cast<const uint32_t&>(d);
 }
 __device__ __forceinline__ uint32_t codes_f16_hi(uint32_t v) {
-  const uint32_t x = (v & 0x00F000F0u) | 0x64006400u;
+  const uint32_t x = and_or(v, 0x00F000F0u, 0x64006400u);
   const __half2 d = __hfma2(reinterpret_cast<const __half2&>(x), __half2half2(__ushort_as_half(0x2C00)),
                             __half2half2(__ushort_as_half(0xD480)));
   return reinterpret_cast<const uint32_t&>(d);
@@ -515,22 +522,23 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
   };
   int64_t rows_cur = rows_of(0), rows_next = my_tiles > 32 ? rows_of(32) : -1;
   constexpr uint32_t kC = kTileKeys * D / 2, kP = kTileKeys * D / 8;  // bytes of a tile's codes and parameters
+  // lanes 0-3 copy one of a tile's four arrays each: where it starts, and its offset in a stage
+  const unsigned char* from = lane == 0 ? p.c.k_codes : lane == 1 ? reinterpret_cast<const unsigned char*>(p.c.k_params)
+                              : lane == 2 ? p.c.v_codes : reinterpret_cast<const unsigned char*>(p.c.v_params);
+  const uint32_t row_bytes = lane & 1 ? D / 8 : D / 2, bytes = row_bytes * kTileKeys;
+  const uint32_t to = smem_u32(ring) + (lane & 1 ? kC : 0u) + (lane & 2 ? kC + kP : 0u);
   auto issue = [&](int it, int base) {  // copies of tile it into stage it % kStages; base: first tile of rows_cur
     const int64_t r = it < base + 32 ? __shfl_sync(0xFFFFFFFFu, rows_cur, it - base)
                                      : __shfl_sync(0xFFFFFFFFu, rows_next, it - base - 32);
-    if (lane == 0) {
-      const int s = it % kStages;
-      const uint32_t bar = bar0 + 8 * s, dst = smem_u32(ring + s * S::kTileBytes);
-      if (r >= 0) {
-        mbar_expect_tx(bar, S::kTileBytes);
-        bulk_load(dst, p.c.k_codes + r * (D / 2), kC, bar);
-        bulk_load(dst + kC, p.c.k_params + r * kG, kP, bar);
-        bulk_load(dst + kC + kP, p.c.v_codes + r * (D / 2), kC, bar);
-        bulk_load(dst + 2 * kC + kP, p.c.v_params + r * kG, kP, bar);
-      } else {
-        mbar_arrive(bar);
-      }
+    const int s = it % kStages;
+    const uint32_t bar = bar0 + 8 * s;
+    if (r < 0) {
+      if (lane == 0) mbar_arrive(bar);
+      return;
     }
+    if (lane == 0) mbar_expect_tx(bar, S::kTileBytes);
+    __syncwarp();
+    if (lane < 4) bulk_load(to + s * S::kTileBytes, from + r * row_bytes, bytes, bar);
   };
 #pragma unroll
   for (int s = 0; s < kStages; ++s)
@@ -731,7 +739,19 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
         }
       }
     }
-    // mask, running maximum
+    if (!whole) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int sl = 0; sl < kSlots; ++sl)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int l = l0 + sl * 16 * KP + own + (i < 2 ? 0 : 8);
+            if (!there || l >= limit[n][i & 1]) sc[sl][n][i] = -INFINITY;
+          }
+      asm volatile("");  // a branch and not a select per score
+    }
+    // running maximum
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float top[2] = {-INFINITY, -INFINITY};
@@ -740,7 +760,6 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int l = l0 + sl * 16 * KP + own + (i < 2 ? 0 : 8);
-          if (!whole) sc[sl][n][i] = there && l < limit[n][i & 1] ? sc[sl][n][i] : -INFINITY;
           top[i & 1] = fmaxf(top[i & 1], sc[sl][n][i]);
           if constexpr (kLogits) {
             const int col = col0 + (KP == 2 ? 2 * (t & 1) : 8 * n + 2 * t) + (i & 1);
@@ -1097,7 +1116,7 @@ static int plan_decode(const sva_kv4_cache* c, const sva_kv4_decode_args* a, Kv4
   plan->n_cols = (int)n_cols;
   plan->col_tiles = (int)tiles;
   const int64_t problems = (int64_t)a->n_seqs * c->n_kv_heads * plan->col_tiles;
-  const int64_t slots = 148 * 5;  // CTAs that fit the GPU at once
+  const int64_t slots = 148 * 4;  // CTAs that fit the GPU at once
   const int64_t tiles_k = std::max<int64_t>(1, (a->max_len + kTileKeys - 1) / kTileKeys);
   int64_t chunks = std::max<int64_t>(1, slots / problems);
   // at least 4 tiles a CTA (one a warp); at most 64 where lengths differ, so that long sequences spread
