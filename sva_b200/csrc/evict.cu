@@ -31,14 +31,21 @@ struct EvictParams {
 // The weights' order as unsigned numbers, NaN above everything.
 __device__ __forceinline__ uint32_t weight_key(float w) { return w != w ? 0xFFFFFFFFu : ordered_key(w); }
 
-// One CTA per (sequence, kv head).  Radix select of the need-th largest weight among the old rows,
-// then one pass in index order: rows above it stay, and of the rows equal to it the first ones.
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictParams p) {
+constexpr int kSelKeys = 49152;  // ordered keys held in shared memory: up to so many old rows are read once
+
+// One CTA per (sequence, kv head).  Radix select of the need-th largest weight among the old rows, then one pass in index
+// order: rows above it stay, and of the rows equal to it the first ones.  A warp owns a stretch of the rows, so that the
+// order needs one scan over the warps and ballots within them.  Latency bound.
+__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictParams p, int room) {
+  extern __shared__ __align__(16) uint32_t keys[];  // [room]
   __shared__ int hist[kBins];
   __shared__ int scratch[kSelThreads / 32 + 1];
+  __shared__ int warp_above[kSelThreads / 32], warp_equal[kSelThreads / 32];
   __shared__ uint32_t s_prefix;
   __shared__ int s_need;
-  const int tid = threadIdx.x, problem = blockIdx.x, b = problem / p.n_kv, h = problem % p.n_kv;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int problem = blockIdx.x, b = problem / p.n_kv, h = problem % p.n_kv;
+  pdl_launch_dependents();
   int64_t n = __ldg(p.seq_lens + b);
   n = n < 0 ? 0 : (n > p.max_len ? p.max_len : n);
   int32_t* kept = p.kept + (int64_t)problem * p.keep;
@@ -55,18 +62,35 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
   if (need == 0) return;
   const float* w = p.weights + b * p.w_seq + h * p.w_head;
 
+  // this warp's rows: first + 32 i + lane, i < steps
+  const int steps = (old + kSelThreads - 1) / kSelThreads;
+  const int64_t first = (int64_t)warp * steps * 32 + lane;
+  const bool held = old <= room;
+  if (held) {
+#pragma unroll 4
+    for (int r = tid; r < old; r += kSelThreads) keys[r] = weight_key(__ldg(w + r));
+    __syncthreads();
+  }
+  // f(key, row, whether there is such a row) for the lane's rows in order, by the whole warp together
+  auto each = [&](auto&& f) {
+#pragma unroll 2
+    for (int i = 0; i < steps; ++i) {
+      const int64_t r = first + 32 * (int64_t)i;
+      const bool there = r < old;
+      f(there ? (held ? keys[r] : weight_key(__ldg(w + r))) : 0u, (int)r, there);
+    }
+  };
+
   uint32_t prefix = 0;
-  const int chosen = need;
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
+    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), above = pass == 1 ? 21 : 10;
     const uint32_t mask = pass == 2 ? 1023u : 2047u;
     for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
     __syncthreads();
-    for (int i = tid; i < old; i += kSelThreads) {
-      const uint32_t k = weight_key(__ldg(w + i));
-      if (pass == 0 || (k >> (pass == 1 ? 21 : 10)) == prefix) atomicAdd(&hist[(k >> shift) & mask], 1);
-    }
+    each([&](uint32_t k, int, bool there) {
+      if (there && (pass == 0 || (k >> above) == prefix)) atomicAdd(&hist[(k >> shift) & mask], 1);
+    });
     __syncthreads();
     // bins from the top: thread i owns bins 2047 - 2i and 2046 - 2i
     const int hi = hist[kBins - 1 - 2 * tid], lo = hist[kBins - 2 - 2 * tid];
@@ -86,17 +110,25 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
   }
   // `prefix` is the need-th largest key; `need` of the rows equal to it stay
   int above = 0, equal = 0;
-  for (int i0 = 0; i0 < old && above + min(equal, need) < chosen; i0 += kSelThreads) {
-    const int i = i0 + tid;
-    const uint32_t k = i < old ? weight_key(__ldg(w + i)) : 0;
-    const int is_above = i < old && k > prefix, is_equal = i < old && k == prefix;
-    int total;
-    const int pre = block_excl_scan(is_above | (is_equal << 16), scratch, &total);
-    const int a = above + (pre & 0xFFFF), e = equal + (pre >> 16);
-    if (is_above || (is_equal && e < need)) kept[a + min(e, need)] = i;
-    above += total & 0xFFFF;
-    equal += total >> 16;
-  }
+  each([&](uint32_t k, int, bool there) {
+    above += __popc(__ballot_sync(0xFFFFFFFFu, there && k > prefix));
+    equal += __popc(__ballot_sync(0xFFFFFFFFu, there && k == prefix));
+  });
+  if (lane == 0) warp_above[warp] = above, warp_equal[warp] = equal;
+  __syncthreads();
+  // rows above and equal to it in the warps before this one
+  const int wa = warp_incl_scan(warp_above[lane]), we = warp_incl_scan(warp_equal[lane]);
+  int at_above = __shfl_sync(0xFFFFFFFFu, wa - warp_above[lane], warp);
+  int at_equal = __shfl_sync(0xFFFFFFFFu, we - warp_equal[lane], warp);
+  const uint32_t before = (1u << lane) - 1u;
+  each([&](uint32_t k, int row, bool there) {
+    const bool is_above = there && k > prefix, is_equal = there && k == prefix;
+    const uint32_t ma = __ballot_sync(0xFFFFFFFFu, is_above), me = __ballot_sync(0xFFFFFFFFu, is_equal);
+    const int a = at_above + __popc(ma & before), e = at_equal + __popc(me & before);
+    if (is_above || (is_equal && e < need)) kept[a + min(e, need)] = row;
+    at_above += __popc(ma);
+    at_equal += __popc(me);
+  });
 }
 
 __device__ __forceinline__ int64_t page_row(const int32_t* table, int64_t stride, int64_t cols, int64_t pages,
@@ -132,6 +164,23 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, const sva_evict_
   };
   V* buf = reinterpret_cast<V*>(smem);
   const int total = (j1 - j0) * units;
+  if (!in_place && units <= kMoveThreads && !p.src_table && !p.dst_table) {
+    // a thread has its place in the row, and takes four rows at a time
+    const int per = kMoveThreads / units, u = threadIdx.x % units;
+    if (threadIdx.x >= per * units || b >= p.src_pages || b >= p.dst_pages) return;
+    const unsigned char* s = static_cast<const unsigned char*>(a.src) + b * a.src_page_stride + h * a.src_head_stride + u * sizeof(V);
+    unsigned char* d = static_cast<unsigned char*>(a.dst) + b * a.dst_page_stride + h * a.dst_head_stride + u * sizeof(V);
+    for (int j = j0 + threadIdx.x / units; j < j1; j += 4 * per) {
+      V v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (j + i * per < j1) v[i] = *reinterpret_cast<const V*>(s + (int64_t)kept[j + i * per] * a.row_bytes);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (j + i * per < j1) *reinterpret_cast<V*>(d + (int64_t)(j + i * per) * a.row_bytes) = v[i];
+    }
+    return;
+  }
   if (!in_place) {
     for (int e = threadIdx.x; e < total; e += kMoveThreads) {
       const int j = j0 + e / units, u = e % units;
@@ -156,11 +205,12 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, const sva_evict_
 // blockIdx.y: the row arrays, then the weights.  Rows move to lower or equal positions, and row j of the
 // result comes from a row >= j: in place, a CTA that owns a whole (array, sequence, head) may take the
 // rows in chunks, reading a chunk before it writes it.
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p, int rows_per_block, bool in_place,
+__global__ void __launch_bounds__(kMoveThreads, 8) evict_move_kernel(const EvictParams p, int rows_per_block, bool in_place,
                                                                   bool weights_in_place) {
   extern __shared__ __align__(16) unsigned char smem[];
   const int problem = blockIdx.z, b = problem / p.n_kv, h = problem % p.n_kv;
   const int which = blockIdx.y;
+  pdl_wait();
   const int stay = p.counts[problem];
   const int32_t* kept = p.kept + (int64_t)problem * p.keep;
   if (which == p.n_arrays) {
@@ -268,7 +318,10 @@ extern "C" int sva_cache_evict(const sva_evict_args* a, const sva_evict_array* a
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int problems = a->n_seqs * a->n_kv_heads;
-  evict_select_kernel<<<problems, kSelThreads, 0, st>>>(p);
+  const int room = (int)std::min<int64_t>(a->max_len, kSelKeys);
+  rc = ensure_smem_attr(reinterpret_cast<const void*>(evict_select_kernel), kSelKeys * 4);
+  if (rc != SVA_OK) return rc;
+  evict_select_kernel<<<problems, kSelThreads, room * 4, st>>>(p, room);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(SVA_ERR_CUDA, cudaGetErrorString(e));
   const bool in_place = a->in_place != 0;
@@ -278,8 +331,18 @@ extern "C" int sva_cache_evict(const sva_evict_args* a, const sva_evict_array* a
   const int rows_per_block = 64;
   const int64_t most = a->keep < a->max_len ? a->keep : a->max_len;
   const int64_t xs = in_place ? 1 : std::max<int64_t>(1, (most + rows_per_block - 1) / rows_per_block);
-  evict_move_kernel<<<dim3((unsigned)xs, a->n_arrays + 1, problems), kMoveThreads, smem, st>>>(p, rows_per_block,
-                                                                                               in_place, w_in_place);
-  e = cudaGetLastError();
+  // launched while the selection drains; it waits there for the selection's memory
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)xs, a->n_arrays + 1, problems);
+  cfg.blockDim = dim3(kMoveThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, evict_move_kernel, p, rows_per_block, in_place, w_in_place);
+  if (e != cudaSuccess) cudaGetLastError();
   return e == cudaSuccess ? SVA_OK : set_error(SVA_ERR_CUDA, cudaGetErrorString(e));
 }

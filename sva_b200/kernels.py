@@ -837,21 +837,29 @@ def kv4_decode(q: torch.Tensor, cache: Kv4Cache, *, seq_lens: torch.Tensor | Non
     return (out, lse) if want_lse else out
 
 
-def _rows_span(t: torch.Tensor, name: str) -> tuple:
+def _rows_span(index: int, t: torch.Tensor, name: str) -> tuple:
     """(first byte, byte behind the last, page stride, head stride, row bytes) of [pages, heads, rows, ...] with
-    contiguous rows."""
-    shape, size = t.shape, t.element_size()
+    contiguous rows, on CUDA device ``index``."""
+    shape, stride, size = t.shape, t.stride(), t.element_size()
     if len(shape) < 3:
         raise ValueError(f"{name} must be [pages, Hkv, page_rows, ...] tensors")
     if t.is_contiguous():
-        row = t.stride(2) * size
+        row = stride[2] * size
     else:
         row = math.prod(shape[3:]) * size
         if 0 not in shape and not t[0, 0].is_contiguous():
             raise ValueError(f"{name} must have contiguous rows")
-    page, head = t.stride(0) * size, t.stride(1) * size
-    at = t.data_ptr()
+    page, head, at = stride[0] * size, stride[1] * size, _there(index, t, name)
     return at, at + (shape[0] - 1) * page + (shape[1] - 1) * head + shape[2] * row, page, head, row
+
+
+def _weights_span(index: int, t: torch.Tensor, name: str, shape: tuple) -> tuple:
+    """(first byte, byte behind the last, sequence stride, head stride) of [B, Hkv, width] sums."""
+    if t.dtype != torch.float32 or t.dim() != 3 or t.shape[:2] != shape or t.stride(2) != 1:
+        raise ValueError(f"{name} must be float32 [B, Hkv, width] with contiguous rows")
+    seq, head, _ = t.stride()
+    at = _there(index, t, name)
+    return at, at + 4 * ((shape[0] - 1) * seq + (shape[1] - 1) * head + t.shape[2]), seq, head
 
 
 def cache_evict(rows: Sequence[torch.Tensor], weights: torch.Tensor, seq_lens: torch.Tensor, keep: int, *,
@@ -887,37 +895,39 @@ def cache_evict(rows: Sequence[torch.Tensor], weights: torch.Tensor, seq_lens: t
     dst_table = page_table if in_place else out_page_table
     n_seqs = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
     like, like_out = src[0].shape[:3], dst[0].shape[:3]
-    spans, packed = [], []
+    read, written, packed = [], [], []
     for s, d in zip(src, dst):
-        one = _rows_span(s, "rows")
-        two = one if in_place else _rows_span(d, "out")
+        one = _rows_span(index, s, "rows")
+        two = one if in_place else _rows_span(index, d, "out")
         if s.shape[:3] != like or d.shape[:3] != like_out:
             raise ValueError("rows must agree in their first three dimensions, and so must out")
         if not in_place and (s.dtype != d.dtype or s.shape[3:] != d.shape[3:]):
             raise ValueError("out must have rows of the same shape and dtype")
-        if _there(index, s, "rows") and _there(index, d, "out"):
-            spans.append((one, two))
+        read.append(one)
+        written.append(two)
         packed.append(_pack_row(one[0], two[0], one[4], one[2], one[3], two[2], two[3]))
     n_kv = like[1]
-    for name, w in (("weights", weights), ("out_weights", dst_weights)):
-        if w.dtype != torch.float32 or w.dim() != 3 or w.shape[:2] != (n_seqs, n_kv) or w.stride(2) != 1:
-            raise ValueError(f"{name} must be float32 [B, Hkv, width] with contiguous rows")
+    w = _weights_span(index, weights, "weights", (n_seqs, n_kv))
+    ow = w if in_place else _weights_span(index, dst_weights, "out_weights", (n_seqs, n_kv))
     if not in_place:
-        w, ow = _rows_span(weights.unsqueeze(3), "weights"), _rows_span(dst_weights.unsqueeze(3), "out_weights")
-        read, written = [one for one, _ in spans] + [w], [two for _, two in spans] + [ow]
-        for i, d in enumerate(written):
-            for other in read + written[:i]:
-                if d[0] < other[1] and other[0] < d[1]:
-                    raise ValueError("out and out_weights must not overlap rows, weights or one another")
+        if like_out[1] != n_kv:
+            raise ValueError("out must have rows' kv heads")
+        # sorted by their first bytes, no range that is written may reach into another
+        spans = sorted([(*x[:2], 0) for x in (*read, w)] + [(*x[:2], 1) for x in (*written, ow)])
+        end, end_written = 0, 0
+        for first, last, out_span in spans:
+            if first < end_written or (out_span and first < end):
+                raise ValueError("out and out_weights must not overlap rows, weights or one another")
+            end = max(end, last)
+            if out_span:
+                end_written = max(end_written, last)
     kept = torch.empty((n_seqs, n_kv, keep), dtype=torch.int32, device=dev)
     lens = torch.empty((n_seqs,), dtype=torch.int64, device=dev)
     table, table_stride, cols = _page_table(index, page_table, n_seqs)
     to, to_stride, to_cols = _page_table(index, dst_table, n_seqs, "out_page_table")
     width = weights.shape[2]
     a = _pack_evict(n_seqs, n_kv, len(src), 1 if in_place else 0, min(width, like[2] * (cols if table else 1)), keep, recent,
-                    _int64(index, seq_lens, "seq_lens", n_seqs), weights.data_ptr(), weights.stride(0), weights.stride(1),
-                    _there(index, dst_weights, "out_weights"), dst_weights.stride(0), dst_weights.stride(1),
-                    dst_weights.shape[2], like[0], like[2], like_out[0], like_out[2], table, table_stride, cols, to,
+                    _int64(index, seq_lens, "seq_lens", n_seqs), w[0], w[2], w[3], ow[0], ow[2], ow[3], dst_weights.shape[2], like[0], like[2], like_out[0], like_out[2], table, table_stride, cols, to,
                     to_stride, to_cols, kept.data_ptr(), lens.data_ptr())
     if n_seqs > 0:
         lib = _lib.load()
