@@ -68,6 +68,11 @@ class SVALlamaServingConfig:
     # scan summon decodes every sequence of a batch in one sva_decode_batched call, each
     # sequence exactly as a batch-1 call would.  Off by default, keeping the reference's error.
     allow_batch: bool = False
+    # Not in the reference, whose prompts go through the summon token by token: "exact" computes calls of
+    # more than one token with attention over every key (sva_prompt_attention) while the catalog is written as
+    # before, so that decode steps still summon.  Unpadded prompts only (no attention mask); such
+    # calls add nothing to the summon counters.
+    prompt_attention: str = "summon"
 
 
 class SVALlamaAttention(nn.Module):
@@ -185,6 +190,30 @@ class SVALlamaAttention(nn.Module):
         return attn_output, None
 
     # ------------------------------------------------------------------------------------
+    def _exact_prompt(self, q_len: int, attention_mask: torch.Tensor | None) -> bool:
+        """Whether this call's tokens attend to every key (serving option ``prompt_attention``)."""
+        mode = self.serving.prompt_attention
+        if mode not in {"summon", "exact"}:
+            raise ValueError(f"Unknown prompt_attention {mode!r}; expected 'summon' or 'exact'.")
+        if mode == "summon" or q_len == 1:
+            return False
+        if attention_mask is not None:
+            raise ValueError("prompt_attention='exact' takes unpadded prompts without an attention mask.")
+        return True
+
+    def _prompt_attention(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, k_len: int) -> torch.Tensor:
+        """query [B, H, q, D] over the first k_len rows of key / value [B, Hkv, >= k_len, D], causal and
+        aligned at the end: [B, H, q, D].  One call a sequence, on views."""
+        batch, n_heads, q_len, head_dim = query.shape
+        both = torch.arange(2, device=query.device)
+        cu, cu_k = both * q_len, both * k_len
+        out = torch.empty(batch, q_len, n_heads, head_dim, dtype=query.dtype, device=query.device)
+        for b in range(batch):
+            kernels.prompt_attention(query[b].transpose(0, 1), key[b, :, :k_len].transpose(0, 1),
+                                     value[b, :, :k_len].transpose(0, 1), cu, cu_seqlens_k=cu_k,
+                                     softmax_scale=self.scaling, out=out[b])
+        return out.transpose(1, 2)
+
     def sva_attention(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                       attention_mask: torch.Tensor | None) -> torch.Tensor:
         """query [1, H, q, D]; key/value [1, Hkv, L, D] (not repeated) -> [1, H, q, D]."""
@@ -200,6 +229,7 @@ class SVALlamaAttention(nn.Module):
         if mode not in {"scan", "inverted", "inverted_static"}:
             raise ValueError(f"Unknown SVA summon_mode: {mode!r}")
         dev = query.device
+        exact = self._exact_prompt(q_len, attention_mask)
         keys = key[0]
         values = value[0]
         if keys.stride(-1) != 1:
@@ -216,6 +246,8 @@ class SVALlamaAttention(nn.Module):
         if ev:
             ev.mark("start")
         self._key_catalog(keys, q_len)
+        if exact:
+            return self._prompt_attention(query, keys.unsqueeze(0), values.unsqueeze(0), k_len)
         if ev:
             ev.mark("catalog")
         counters = None if self.stats is None else self.stats.device_counters(int(self.layer_idx or 0), dev)
@@ -314,8 +346,11 @@ class SVALlamaAttention(nn.Module):
         # prefill (not captured): positions and lengths on the host
         first, last = int(pos[0]), int(pos[-1])
         k_len = last + 1
+        exact = self._exact_prompt(q_len, None)
         kernels.catalog_encode(flat_keys, self._srep[0], self._srep[1], first, k_len - first, flat_low, flat_codes,
                                n_heads=batch * n_heads)
+        if exact:
+            return self._prompt_attention(query, key, value, k_len)
         out = torch.empty(batch, n_heads, q_len, head_dim, dtype=query.dtype, device=dev)
         chunk = q_len
         if _grid_schedule(k_len, self.serving.coarse_shortlist, self.serving.budget):
@@ -352,7 +387,10 @@ class SVALlamaAttention(nn.Module):
             key = key.contiguous()
         if value.stride(-1) != 1:
             value = value.contiguous()
+        exact = self._exact_prompt(q_len, attention_mask)
         self._key_catalog_batched(key, q_len)
+        if exact:
+            return self._prompt_attention(query, key, value, k_len)
         allowed_mask = None
         if attention_mask is not None:
             m = attention_mask[..., :q_len, :k_len] > -1e4
@@ -569,7 +607,8 @@ class SVALlamaPatcher:
                  adaptive_min_budget: int | None = None, adaptive_mid_budget: int | None = None,
                  adaptive_low_margin: float = 0.35, adaptive_high_margin: float = 0.70,
                  profile_components: bool = False, static_tail_rebuild_interval: int = 64,
-                 layers: list[int] | None = None, write_path: str = "exact", allow_batch: bool = False) -> None:
+                 layers: list[int] | None = None, write_path: str = "exact", allow_batch: bool = False,
+                 prompt_attention: str = "summon") -> None:
         self.model = model
         self.bundle = bundle
         self.stats = SVAStats()
@@ -591,6 +630,7 @@ class SVALlamaPatcher:
             static_tail_rebuild_interval=static_tail_rebuild_interval,
             write_path=write_path,
             allow_batch=allow_batch,
+            prompt_attention=prompt_attention,
         )
 
     def patch(self) -> "SVALlamaPatcher":
@@ -668,14 +708,16 @@ def patch_llama_attention(model: nn.Module, artifact_dir_or_bundle: str | Path |
                           adaptive_mid_budget: int | None = None, adaptive_low_margin: float = 0.35,
                           adaptive_high_margin: float = 0.70, profile_components: bool = False,
                           static_tail_rebuild_interval: int = 64, layers: list[int] | None = None,
-                          write_path: str = "exact", allow_batch: bool = False) -> SVALlamaPatcher:
+                          write_path: str = "exact", allow_batch: bool = False,
+                          prompt_attention: str = "summon") -> SVALlamaPatcher:
     """Patch a Llama-family model with SVA attention and return a reversible handle (reference sva/llama.py:808-848).
 
     ``write_path`` (not in the reference) selects the key projection: "exact" (default; CUDA cores,
     canonical fp32 order, bit-exact codes) or "auto" (tcgen05 tensor cores when the keys are bf16
     and the projection holds bf16 values; codes may flip at near ties).  ``allow_batch`` (not in the
     reference, which raises on batch != 1) decodes batches of sequences in one call per layer in
-    scan mode, each sequence exactly as at batch 1.
+    scan mode, each sequence exactly as at batch 1.  ``prompt_attention`` (not in the reference) "exact" lets calls of more
+    than one token attend to every key, at the speed of the packed prompt kernel; decode steps summon as before.
     """
     bundle = (artifact_dir_or_bundle if isinstance(artifact_dir_or_bundle, SVAArtifactBundle)
               else load_sva_artifact_bundle(artifact_dir_or_bundle))
@@ -686,5 +728,5 @@ def patch_llama_attention(model: nn.Module, artifact_dir_or_bundle: str | Path |
         adaptive_mid_budget=adaptive_mid_budget, adaptive_low_margin=adaptive_low_margin,
         adaptive_high_margin=adaptive_high_margin, profile_components=profile_components,
         static_tail_rebuild_interval=static_tail_rebuild_interval, layers=layers, write_path=write_path,
-        allow_batch=allow_batch,
+        allow_batch=allow_batch, prompt_attention=prompt_attention,
     ).patch()
