@@ -838,8 +838,8 @@ def kv4_decode(q: torch.Tensor, cache: Kv4Cache, *, seq_lens: torch.Tensor | Non
 
 
 def _rows_span(index: int, t: torch.Tensor, name: str) -> tuple:
-    """(first byte, byte behind the last, page stride, head stride, row bytes) of [pages, heads, rows, ...] with
-    contiguous rows, on CUDA device ``index``."""
+    """(first byte, byte behind the last, page stride, head stride, row bytes, bytes that a page spans) of [pages, heads,
+    rows, ...] with contiguous rows, on CUDA device ``index``."""
     shape, stride, size = t.shape, t.stride(), t.element_size()
     if len(shape) < 3:
         raise ValueError(f"{name} must be [pages, Hkv, page_rows, ...] tensors")
@@ -850,7 +850,8 @@ def _rows_span(index: int, t: torch.Tensor, name: str) -> tuple:
         if 0 not in shape and not t[0, 0].is_contiguous():
             raise ValueError(f"{name} must have contiguous rows")
     page, head, at = stride[0] * size, stride[1] * size, _there(index, t, name)
-    return at, at + (shape[0] - 1) * page + (shape[1] - 1) * head + shape[2] * row, page, head, row
+    within = (shape[1] - 1) * head + shape[2] * row
+    return at, at + (shape[0] - 1) * page + within, page, head, row, within
 
 
 def _weights_span(index: int, t: torch.Tensor, name: str, shape: tuple) -> tuple:
@@ -860,6 +861,31 @@ def _weights_span(index: int, t: torch.Tensor, name: str, shape: tuple) -> tuple
     seq, head, _ = t.stride()
     at = _there(index, t, name)
     return at, at + 4 * ((shape[0] - 1) * seq + (shape[1] - 1) * head + t.shape[2]), seq, head
+
+
+def _apart(a: tuple, b: tuple) -> bool:
+    """Whether two strided arrays of one page stride (keys and values side by side in every page) lie apart."""
+    page = a[2]
+    if len(a) < 6 or len(b) < 6 or page != b[2] or page <= 0:
+        return False
+    gap = (b[0] - a[0]) % page
+    return gap >= a[5] and gap + b[5] <= page
+
+
+def _spans_meet(read: list, written: list) -> bool:
+    """Whether an array of ``written`` overlaps another of ``written`` or one of ``read``."""
+    spans = sorted([(x[0], x[1], 0) for x in read] + [(x[0], x[1], 1) for x in written])
+    end = end_written = 0
+    for first, last, out in spans:
+        if first < end_written or (out and first < end):
+            break
+        end = max(end, last)
+        if out:
+            end_written = max(end_written, last)
+    else:
+        return False
+    return any(x[0] < y[1] and y[0] < x[1] and not _apart(x, y)
+               for i, x in enumerate(written) for y in (*read, *written[:i]))
 
 
 def cache_evict(rows: Sequence[torch.Tensor], weights: torch.Tensor, seq_lens: torch.Tensor, keep: int, *,
@@ -874,7 +900,7 @@ def cache_evict(rows: Sequence[torch.Tensor], weights: torch.Tensor, seq_lens: t
     the largest).  Rows that stay move together in their order, with their weights; weights behind them
     become 0.  In place, unless ``out`` (and then ``out_weights``, ``out_page_table``) name another cache; in place no
     page may belong to two sequences.  Returns (kept [B, Hkv, keep] int32: the old positions, ascending,
-    -1 padded; lengths [B] int64).  Append new rows at the returned lengths, and keep the model's own position
+    -1 padded; lengths [B] int64).  What is written may overlap nothing else.  Append new rows at the returned lengths, and keep the model's own position
     count for rotary embeddings: rows are not re-rotated.
     """
     if not weights.is_cuda:
@@ -909,26 +935,20 @@ def cache_evict(rows: Sequence[torch.Tensor], weights: torch.Tensor, seq_lens: t
     n_kv = like[1]
     w = _weights_span(index, weights, "weights", (n_seqs, n_kv))
     ow = w if in_place else _weights_span(index, dst_weights, "out_weights", (n_seqs, n_kv))
-    if not in_place:
-        if like_out[1] != n_kv:
-            raise ValueError("out must have rows' kv heads")
-        # sorted by their first bytes, no range that is written may reach into another
-        spans = sorted([(*x[:2], 0) for x in (*read, w)] + [(*x[:2], 1) for x in (*written, ow)])
-        end, end_written = 0, 0
-        for first, last, out_span in spans:
-            if first < end_written or (out_span and first < end):
-                raise ValueError("out and out_weights must not overlap rows, weights or one another")
-            end = max(end, last)
-            if out_span:
-                end_written = max(end_written, last)
+    if like_out[1] != n_kv:
+        raise ValueError("out must have rows' kv heads")
+    if _spans_meet([] if in_place else [*read, w], [*written, ow]):
+        raise ValueError("rows and weights that are written must not overlap one another" if in_place else
+                         "out and out_weights must not overlap rows, weights or one another")
     kept = torch.empty((n_seqs, n_kv, keep), dtype=torch.int32, device=dev)
     lens = torch.empty((n_seqs,), dtype=torch.int64, device=dev)
     table, table_stride, cols = _page_table(index, page_table, n_seqs)
     to, to_stride, to_cols = _page_table(index, dst_table, n_seqs, "out_page_table")
     width = weights.shape[2]
     a = _pack_evict(n_seqs, n_kv, len(src), 1 if in_place else 0, min(width, like[2] * (cols if table else 1)), keep, recent,
-                    _int64(index, seq_lens, "seq_lens", n_seqs), w[0], w[2], w[3], ow[0], ow[2], ow[3], dst_weights.shape[2], like[0], like[2], like_out[0], like_out[2], table, table_stride, cols, to,
-                    to_stride, to_cols, kept.data_ptr(), lens.data_ptr())
+                    _int64(index, seq_lens, "seq_lens", n_seqs), w[0], w[2], w[3], ow[0], ow[2], ow[3],
+                    dst_weights.shape[2], like[0], like[2], like_out[0], like_out[2], table, table_stride, cols, to, to_stride,
+                    to_cols, kept.data_ptr(), lens.data_ptr())
     if n_seqs > 0:
         lib = _lib.load()
         nbytes = lib.sva_cache_evict_workspace_size(a)

@@ -593,6 +593,129 @@ def test_cache_evict_order_of_awkward_weights():
         assert out.flatten().tolist() == want
 
 
+def test_cache_evict_keys_and_values_side_by_side():
+    """Keys and values as views of one pool [pages, 2, Hkv, rows, D], and the refusal of arrays that do overlap."""
+    from sva_b200 import kernels
+
+    g = _gen(5)
+    pool = _randn(g, 2, 2, 3, 64, 32, dtype=torch.bfloat16)
+    before, w = pool.clone(), torch.rand(2, 3, 64, generator=g, device=DEV)
+    n = torch.tensor([64, 40], device=DEV)
+    w0 = w.clone()
+    kept, lens = kernels.cache_evict([pool[:, 0], pool[:, 1]], w, n, 16, recent=4)
+    for b in range(2):
+        for h in range(3):
+            at = torch.tensor(_kept(w0[b, h], int(n[b]), 16, 4), device=DEV)
+            assert torch.equal(kept[b, h].long(), at)
+            assert torch.equal(pool[b, :, h, :16], before[b, :, h, at])
+            assert torch.equal(pool[b, :, h, 16:], before[b, :, h, 16:])
+    out, ow = torch.zeros(2, 2, 3, 16, 32, dtype=torch.bfloat16, device=DEV), torch.zeros(2, 3, 16, device=DEV)
+    kernels.cache_evict([pool[:, 0], pool[:, 1]], w, n, 16, out=[out[:, 0], out[:, 1]], out_weights=ow)
+    keys = pool[:, 0]
+    for bad in (lambda: kernels.cache_evict([keys, keys], w, n, 16),
+                lambda: kernels.cache_evict([keys[:, :, :40], keys[:, :, 8:48]], w, n, 16),
+                lambda: kernels.cache_evict([keys], w, n, 16, out=[keys], out_weights=ow),
+                lambda: kernels.cache_evict([keys], w, n, 16, out=[out[:, 0]], out_weights=w),
+                lambda: kernels.cache_evict([keys, keys], w, n, 16, out=[out[:, 0], out[:, 0]], out_weights=ow)):
+        with pytest.raises(ValueError, match="overlap"):
+            bad()
+
+
+@pytest.mark.parametrize("dim", [8, 24, 40, 56, 72, 104, 120])
+def test_prompt_head_dims_that_fill_part_of_a_tile(dim):
+    from sva_b200 import kernels
+
+    q, k, v, cu, cu_k = _prompt_case([150, 1, 20], [150, 1, 300], 6, 2, dim, torch.bfloat16, seed=dim)
+    _check_prompt(q, k, v, cu, cu_k, *kernels.prompt_attention(q, k, v, cu, cu_seqlens_k=cu_k, want_lse=True))
+
+
+def test_prompt_split_over_a_long_axis():
+    """Few rows over many keys: the keys are shared out and joined; rows that see nothing, and NaN, come through."""
+    from sva_b200 import kernels
+
+    q, k, v, cu, cu_k = _prompt_case([5, 9], [5000, 3], 8, 2, 64, torch.bfloat16, seed=8)
+    out, lse = kernels.prompt_attention(q, k, v, cu, cu_seqlens_k=cu_k, want_lse=True)
+    _check_prompt(q, k, v, cu, cu_k, out, lse)
+    k[4000, 0] = float("nan")
+    v[4998, 1, 3] = float("nan")  # seen by the last two queries of the first sequence
+    got = kernels.prompt_attention(q, k, v, cu, cu_seqlens_k=cu_k)
+    assert bool(got[:5, :4].isnan().all())
+    bad = torch.zeros_like(got[:, 4:], dtype=torch.bool)
+    bad[3:5, :, 3] = True
+    assert torch.equal(got[:, 4:].isfinite(), ~bad)
+    assert torch.equal(got[:, 4:][~bad], out[:, 4:][~bad])
+
+
+def test_kv4_decode_scales_of_very_different_size():
+    """Values whose scales span 2^40, in an order that makes the running bound grow, and tiny and huge queries."""
+    from sva_b200 import kernels
+
+    q, cache, _, n, rows, longest = _decode_case([700], 3, 1, 64, 1, torch.bfloat16, 0, seed=11)
+    size = torch.ones(700, device=DEV)
+    size[:256], size[256:512], size[600:] = 2.0 ** -30, 2.0 ** -10, 2.0 ** 10
+    v = (rows[1].float() * size[:, None]).to(torch.bfloat16)
+    kernels.kv4_write(rows[0], v, cache, torch.zeros(1, dtype=torch.int64, device=DEV))
+    for factor in (1.0, 2.0 ** -40, 2.0 ** 30):
+        out = kernels.kv4_decode(q * factor, cache, seq_lens=n, max_len=longest, softmax_scale=0.125 / factor)
+        _check_decode(q, (rows[0], v), n, out, scale=0.125)
+    # a scale of zero weighs every key alike; a negative one is the positive one of -q
+    assert torch.equal(kernels.kv4_decode(q, cache, seq_lens=n, max_len=longest, softmax_scale=-0.125),
+                       kernels.kv4_decode(-q, cache, seq_lens=n, max_len=longest, softmax_scale=0.125))
+    _check_decode(q * 0, (rows[0], v), n, kernels.kv4_decode(q, cache, seq_lens=n, max_len=longest, softmax_scale=0.0))
+
+
+def test_kv4_decode_non_finite_groups_stay_in_their_channels():
+    from sva_b200 import kernels
+
+    q, cache, _, n, rows, longest = _decode_case([300], 3, 1, 64, 1, torch.bfloat16, 0, seed=13)
+    want = kernels.kv4_decode(q, cache, seq_lens=n, max_len=longest)
+    rows[1][0, 0, 250, 40] = float("inf")
+    kernels.kv4_write(rows[0][:, :, 250:251], rows[1][:, :, 250:251], cache, torch.tensor([250], device=DEV))
+    got = kernels.kv4_decode(q, cache, seq_lens=n, max_len=longest)
+    assert bool(got[..., 32:].isnan().all()) and torch.equal(got[..., :32], want[..., :32])
+    assert torch.equal(kernels.kv4_decode(q, cache, seq_lens=n - 50, max_len=longest),
+                       kernels.kv4_decode(q, cache, seq_lens=n - 50, max_len=longest).nan_to_num(7.0))
+
+
+def test_wrapper_refusals():
+    from sva_b200 import kernels
+
+    q, k, v, cu, _ = _prompt_case([10], [10], 4, 2, 64, torch.bfloat16)
+    for call, error in ((lambda: kernels.prompt_attention(q[0], k, v, cu), ValueError),
+                        (lambda: kernels.prompt_attention(q, k.half(), v, cu), TypeError),
+                        (lambda: kernels.prompt_attention(q, k[:5], v[:5], cu), ValueError),
+                        (lambda: kernels.prompt_attention(q, k[..., :32], v[..., :32], cu), ValueError),
+                        (lambda: kernels.prompt_attention(q, k, v, cu.int()), ValueError),
+                        (lambda: kernels.prompt_attention(q, k, v, cu.cpu()), RuntimeError),
+                        (lambda: kernels.prompt_attention(q[:, :3], k, v, cu), ValueError),
+                        (lambda: kernels.prompt_attention(q.double(), k.double(), v.double(), cu), TypeError),
+                        (lambda: kernels.prompt_attention(q, k, v, cu, out=q[:5]), ValueError)):
+        with pytest.raises(error):
+            call()
+    dq, cache, table, n, rows, longest = _decode_case([70, 64], 4, 2, 64, 1, torch.bfloat16, 64, seed=1)
+    for call, error in ((lambda: kernels.kv4_decode(dq[0], cache), ValueError),
+                        (lambda: kernels.kv4_decode(dq[..., :32], cache), ValueError),
+                        (lambda: kernels.kv4_decode(dq[:, :3], cache, page_table=table), ValueError),
+                        (lambda: kernels.kv4_decode(dq, cache, page_table=table[:1]), ValueError),
+                        (lambda: kernels.kv4_decode(dq, cache, page_table=table.long()), ValueError),
+                        (lambda: kernels.kv4_decode(dq, cache, page_table=table, max_len=129), ValueError),
+                        (lambda: kernels.kv4_decode(dq, cache, page_table=table, seq_lens=n.int()), ValueError),
+                        (lambda: kernels.kv4_decode(dq, cache, page_table=table, weights=torch.zeros(2, 2, 9, device=DEV)),
+                         ValueError),
+                        (lambda: kernels.kv4_write(rows[0], rows[1][:, :1], cache, n), ValueError),
+                        (lambda: kernels.kv4_write(rows[0], rows[1].half(), cache, n), TypeError),
+                        (lambda: kernels.kv4_write(rows[0], rows[1], cache, n[:1]), ValueError),
+                        (lambda: kernels.kv4_read(cache, n, -1), ValueError),
+                        (lambda: kernels.kv4_read(cache, n, 1, dtype=torch.int8), TypeError),
+                        (lambda: kernels.cache_evict(cache, torch.zeros(2, 2, 128, device=DEV), n, -1, page_table=table),
+                         ValueError),
+                        (lambda: kernels.cache_evict(cache, torch.zeros(2, 2, 128, device=DEV), n, 9, recent=10,
+                                                     page_table=table), ValueError),
+                        (lambda: kernels.cache_evict([], torch.zeros(2, 2, 128, device=DEV), n, 9), ValueError)):
+        with pytest.raises(error):
+            call()
+
+
 # ------------------------------------------------------------------------------------------
 # all of them together, streams, graphs, large offsets
 # ------------------------------------------------------------------------------------------
