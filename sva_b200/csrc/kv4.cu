@@ -551,14 +551,28 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
   for (int n = 0; n < NT; ++n) {
     const int col = col0 + (KP == 2 ? (g & 3) : 8 * n + g);
     const bool live = col < p.n_cols;
-    const int tok = col / p.groups, head = h * p.groups + col % p.groups;
+    const int tok = p.n_tokens == 1 ? 0 : col / p.groups, head = h * p.groups + col - tok * p.groups;
     const T* src = reinterpret_cast<const T*>(p.q) + b * p.q_seq + (int64_t)head * p.q_head + (int64_t)tok * p.q_row;
     float x[kG][8], big = 0.f, unit = 1.f;
+    const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+#pragma unroll
+    for (int gr = 0; gr < kG; ++gr) {
+      uint4 raw[sizeof(T) / 2] = {};
+      const T* at = src + gr * kGroup + 8 * t;
+      if (live && vec) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(at) + i);
+      } else if (live) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(raw)[i] = at[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[gr][i] = to_f32<T>(reinterpret_cast<const T*>(raw)[i]);
+    }
 #pragma unroll
     for (int gr = 0; gr < kG; ++gr)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[gr][i] = live ? to_f32<T>(src[gr * kGroup + 8 * t + i]) : 0.f;
         if (p.scale_log2 < 0.f) x[gr][i] = -x[gr][i];  // the scale below is then positive
         big = fmaxf(big, fabsf(x[gr][i]));
       }
@@ -611,7 +625,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int col = col0 + (KP == 2 ? 2 * (t & 1) : 8 * n + 2 * t) + j;
-      const int64_t seen = len - p.n_tokens + col / p.groups + 1 - key0;
+      const int64_t seen = len - p.n_tokens + (p.n_tokens == 1 ? 0 : col / p.groups) + 1 - key0;
       limit[n][j] = col < p.n_cols ? (int)min(max(seen, (int64_t)0), p.chunk_keys) : 0;
     }
   // keys that every column sees, and that any sees
@@ -933,7 +947,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
       o = any_failed ? NAN : fmaf(f, w_o[(w * S::kCols + c) * D + d], o);
     }
     if (last) {
-      const int tok = col / p.groups, head = h * p.groups + col % p.groups;
+      const int tok = p.n_tokens == 1 ? 0 : col / p.groups, head = h * p.groups + col - tok * p.groups;
       const bool none = top == -INFINITY && l == 0.f;
       reinterpret_cast<T*>(p.out)[b * p.o_seq + (int64_t)head * p.o_head + (int64_t)tok * p.o_row + d] =
           from_f32<T>(none ? 0.f : o / l);
@@ -998,7 +1012,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Kv4DecPara
     if (tid < D) {
 #pragma unroll
       for (int i = 1; i < kJoinThreads / D; ++i) o += part[tid + i * D];
-      const int tok = col / p.groups, head = h * p.groups + col % p.groups;
+      const int tok = p.n_tokens == 1 ? 0 : col / p.groups, head = h * p.groups + col - tok * p.groups;
       const bool none = top == -INFINITY && l == 0.f;
       reinterpret_cast<T*>(p.out)[b * p.o_seq + (int64_t)head * p.o_head + (int64_t)tok * p.o_row + tid] =
           from_f32<T>(none ? 0.f : o / l);
