@@ -68,7 +68,8 @@ __device__ __forceinline__ bool find_tile(const PromptParams& p, int64_t slot, i
 // ---------------------------------------------------------------------------------------
 // One CTA takes 64 queries of one head and walks the keys in tiles of 64 with a running maximum and
 // sum per row; a thread owns 4 rows x 4 keys of the scores and 4 rows x D / 16 channels of the output.
-// Bound by fp32 issue: 4 D flops a (query, key) pair at 2 x 128 lanes a cycle and SM.
+// Bound by fp32 issue: 4 D flops a (query, key) pair at 2 x 128 lanes a cycle and SM; 8192 tokens of 9 / 3 heads of 64 took
+// 3.1 ms (25 TFLOP/s).
 constexpr int kSimtRows = 64;
 
 template <typename T, int DP>
@@ -206,11 +207,14 @@ __global__ void __launch_bounds__(256) prompt_simt_kernel(const PromptParams p) 
 // fill a tile.  Roles: warps 0-3 and 4-7 the softmax of A and of B (a thread owns a row), warp 8 the copies,
 // warp 9 the MMAs, warps 10 and 11 the value rows that some row may not see.
 //   S = Q K^T   128 x 128 x D, both operands in shared memory, S in tensor memory (fp32)
-//   P = exp2(scale log2e S - m), written over S as 16-bit numbers
+//   P = exp2(scale log2e S - m) as 16-bit numbers in tensor memory: beside S (D = 64), or over it (D = 128)
 //   O += P V    128 x D x 128, P in tensor memory
 // While one tile is in its softmax the tensor cores work for the other.  The maximum m that P is relative to
 // moves only when a row's maximum grew by more than 2^8 (P stays below 256, well inside fp16), so O is
 // rescaled rarely.
+// Measured (device): 8192 tokens, 9 / 3 heads of 64, bf16: 119 us = 652 TFLOP/s of the causal half; 2 x 61 tokens behind 30011
+// keys, 16 / 2 heads of 128: 52 us.  With 64 channels the exponential unit (16 a cycle and SM, 1024 cycles a tile and block
+// against 512 of MMAs) bounds it and is about 76 % busy: a block of both tiles takes about 2700 cycles.
 constexpr int kTcRows = 128;   // rows of a tile, keys of a block
 constexpr int kTcThreads = 384;
 
