@@ -594,11 +594,12 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[gr][i] *= factor;
     }
-    // this lane accumulates columns 2t and 2t + 1 (mod 4).  A scale of 0 would make NaN of a masked -inf.
+    // this lane accumulates columns 2t and 2t + 1 (mod 4).  A factor of 0 would make NaN of a masked -inf; the smallest normal
+    // number makes 0 of every score just as well.
     const int c = KP == 2 ? 2 * (t & 1) : 2 * t;
-    const float to_log2 = fmaxf(fabsf(p.scale_log2), 1e-37f);
-    scale[n][0] = to_log2 * __shfl_sync(0xFFFFFFFFu, unit, c * 4);
-    scale[n][1] = to_log2 * __shfl_sync(0xFFFFFFFFu, unit, (c + 1) * 4);
+    const float to_log2 = fabsf(p.scale_log2);
+    scale[n][0] = fmaxf(to_log2 * __shfl_sync(0xFFFFFFFFu, unit, c * 4), 1.2e-38f);
+    scale[n][1] = fmaxf(to_log2 * __shfl_sync(0xFFFFFFFFu, unit, (c + 1) * 4), 1.2e-38f);
 #pragma unroll
     for (int gr = 0; gr < kG; ++gr) {
       float sum = 0.f;

@@ -664,6 +664,18 @@ def test_kv4_decode_scales_of_very_different_size():
     _check_decode(q * 0, (rows[0], v), n, kernels.kv4_decode(q, cache, seq_lens=n, max_len=longest, softmax_scale=0.0))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_kv4_decode_zero_queries_and_vanishing_scales(dtype):
+    """Every key weighs the same, in a tile that the sequence ends in too."""
+    from sva_b200 import kernels
+
+    q, cache, _, n, rows, longest = _decode_case([300], 3, 1, 64, 1, dtype, 0, seed=14)
+    zero = torch.zeros_like(q)
+    for query, scale in ((zero, 0.125), (zero, 0.0), (zero, 1e-30), (q, 0.0), (q, 1e-38), (zero, -1e-30)):
+        out = kernels.kv4_decode(query, cache, seq_lens=n, max_len=longest, softmax_scale=scale)
+        _check_decode(zero, rows, n, out)
+
+
 def test_kv4_decode_non_finite_groups_stay_in_their_channels():
     from sva_b200 import kernels
 
