@@ -342,8 +342,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
 //   q.k     = sum_g s_g (q_g . (c_g - 8)) + z_g sum(q_g)
 //   sum p v = sum_g [ (p s_g) . (c_g - 8) ] + sum_keys p z_g
 // so the tensor cores multiply whole numbers and the scales act on fp32 accumulators.  Roundings: none of 16-bit queries (but
-// see the query fragments); p s to fp16 for 16-bit queries, 2^-12 of it (bf16, 2^-9, would show in fp16 outputs), at most 1 by
-// the running lift; fp32 queries and their p s in three bf16 parts, 2^-24 or better.
+// see the query fragments); p s to fp16 for 16-bit queries, 2^-11 of it (bf16, 2^-8, would show in fp16 outputs), at most 1 by
+// the running unit; fp32 queries and their p s in three bf16 parts, 2^-24 or better.
 //
 // Layout.  mma.m16n8k16 with the cache as the 16-row operand and the columns as N: keys x channels for
 // the scores, channels x keys for the output, because a decode step has few columns (heads of a
@@ -638,11 +638,13 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
   const int seen_all = (int)min(max(len - p.n_tokens + 1 - key0, (int64_t)0), p.chunk_keys);
   const int seen_any = (int)(key1 - key0);
 
-  // m_run: the largest scaled score so far; weights are taken relative to m_run + lift.  fp16 weights times scales: lift is the
-  // exponent above the largest scale of V so far (the same for the warp's columns), so that no product passes 1.
+  // m_run: the largest scaled score so far; weights are taken relative to it.  fp16 weights times scales: scales are taken in
+  // units of a power of two above the largest scale of V so far (the same for the warp's columns), so that no product passes 1, and
+  // the accumulators in units of it too.  While every scale is 0, so are the products, in any unit.
   float m_run[NT][2], l_run[NT][2], zsum[kG][NT][2], acc[kG][2][NT][4];
-  float lift = 0.f;
-  uint32_t scale_bound = 0;  // bf16 bits of 2^lift
+  uint32_t scale_bound = 127u << 7;  // bf16 bits of the unit
+  bool unset = true;                 // no scale but 0 so far
+  float per_unit = 1.f;              // 1 / unit
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -738,7 +740,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
       }
     }
     // a scale of V above the bound?  (NaN groups do not count: they make their own channels NaN)
-    bool lifted = false;
+    float rescale = 1.f;  // old unit / new one
     if constexpr (!S::kWide) {
       uint32_t most = 0;
 #pragma unroll
@@ -746,16 +748,19 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
         const uint4 w = *reinterpret_cast<const uint4*>(vp + 16 * (lane + 32 * i));
         most = max(most, max(max(w.x & 0xFFFFu, w.y & 0xFFFFu), max(w.z & 0xFFFFu, w.w & 0xFFFFu)));
       }
-      if (__any_sync(0xFFFFFFFFu, most > scale_bound)) {
+      if (__any_sync(0xFFFFFFFFu, most > (unset ? 0u : scale_bound))) {
         most = 0;
         for (int e = lane; e < kTileKeys * kG; e += 32) {
           const uint32_t w = reinterpret_cast<const uint32_t*>(vp)[e] & 0xFFFFu;
           most = max(most, w < 0x7F80u ? w : 0u);
         }
         most = __reduce_max_sync(0xFFFFFFFFu, most);
-        if (most > scale_bound) {
-          scale_bound = min(max((most >> 7) + 1, 27u), 227u) << 7;
-          lifted = true;
+        if (most > (unset ? 0u : scale_bound)) {
+          const uint32_t e = min(max((most >> 7) + 1, 27u), 227u);
+          rescale = unset ? 1.f : ex2(static_cast<float>(static_cast<int>(scale_bound >> 7) - static_cast<int>(e)));
+          scale_bound = e << 7;
+          per_unit = __uint_as_float((254u - e) << 23);
+          unset = false;
         }
       }
     }
@@ -794,29 +799,27 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
         for (int o = KP == 2 ? 2 : 4; o < 32; o <<= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xFFFFFFFFu, top[j], o));
         top[j] *= scale[n][j];
       }
-      if (__any_sync(0xFFFFFFFFu, lifted || top[0] > m_run[n][0] || top[1] > m_run[n][1])) {
-        const float now = S::kWide ? 0.f : static_cast<float>(static_cast<int>(scale_bound >> 7) - 127);
+      if (__any_sync(0xFFFFFFFFu, rescale != 1.f || top[0] > m_run[n][0] || top[1] > m_run[n][1])) {
         float alpha[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const float m_new = fmaxf(m_run[n][j], top[j]);
-          alpha[j] = m_new == -INFINITY ? 0.f : ex2((m_run[n][j] - m_new) + (lift - now));
+          alpha[j] = m_new == -INFINITY ? 0.f : ex2(m_run[n][j] - m_new);
           m_run[n][j] = m_new;
           l_run[n][j] *= alpha[j];
         }
-        if (n == NT - 1) lift = now;
 #pragma unroll
         for (int gr = 0; gr < kG; ++gr) {
           zsum[gr][n][0] *= alpha[0];
           zsum[gr][n][1] *= alpha[1];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) acc[gr][i >> 2][n][i & 3] *= alpha[i & 1];
+          for (int i = 0; i < 8; ++i) acc[gr][i >> 2][n][i & 3] *= alpha[i & 1] * rescale;
         }
       }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float use[2] = {m_run[n][0] == -INFINITY ? 0.f : m_run[n][0] + lift, m_run[n][1] == -INFINITY ? 0.f : m_run[n][1] + lift};
+      const float use[2] = {m_run[n][0] == -INFINITY ? 0.f : m_run[n][0], m_run[n][1] == -INFINITY ? 0.f : m_run[n][1]};
 #pragma unroll
       for (int sl = 0; sl < kSlots; ++sl)
 #pragma unroll
@@ -837,13 +840,14 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
       for (int gr = 0; gr < kG; ++gr) {
         const float sa = bf16_lo(pa[gr]), sb = bf16_lo(pb[gr]);
         const float za = fmaf(8.f, sa, bf16_hi(pa[gr])), zb = fmaf(8.f, sb, bf16_hi(pb[gr]));
+        const float ua = S::kWide ? sa : sa * per_unit, ub = S::kWide ? sb : sb * per_unit;
         uint32_t bp[NT][S::kParts][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float ps[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            ps[i] = sc[sl][n][i] * (i < 2 ? sa : sb);
+            ps[i] = sc[sl][n][i] * (i < 2 ? ua : ub);
             zsum[gr][n][i & 1] = fmaf(sc[sl][n][i], i < 2 ? za : zb, zsum[gr][n][i & 1]);
           }
 #pragma unroll
@@ -919,7 +923,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
       }
       const int c = (KP == 2 ? 2 * (t & 1) : 8 * n + 2 * t) + j;
       if (g == 0 && (KP == 1 || t < 2)) {
-        w_m[warp][c] = m_run[n][j] + lift;
+        w_m[warp][c] = m_run[n][j];
         w_l[warp][c] = l_run[n][j];
       }
 #pragma unroll
@@ -928,6 +932,11 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
         if constexpr (KP == 2) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[i] += __shfl_xor_sync(0xFFFFFFFFu, o[i], 2);
+        }
+        if constexpr (!S::kWide) {
+          const float unit = __uint_as_float(scale_bound << 16);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] *= unit;
         }
         const float z = zsum[gr][n][j];
         if (!any_failed && (KP == 1 || t < 2))
