@@ -342,8 +342,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
 //   q.k     = sum_g s_g (q_g . (c_g - 8)) + z_g sum(q_g)
 //   sum p v = sum_g [ (p s_g) . (c_g - 8) ] + sum_keys p z_g
 // so the tensor cores multiply whole numbers and the scales act on fp32 accumulators.  Roundings: none of 16-bit queries (but
-// see the query fragments); p s to fp16 for 16-bit queries, 2^-11 of it (bf16, 2^-8, would show in fp16 outputs), at most 1 by
-// the running unit; fp32 queries and their p s in three bf16 parts, 2^-24 or better.
+// see the query fragments); p s to fp16 for 16-bit queries, 2^-11 of it (bf16, 2^-8, would show in fp16 outputs), kept in
+// range by a running unit for each channel group; fp32 queries and their p s in three bf16 parts, 2^-24 or better.
 //
 // Layout.  mma.m16n8k16 with the cache as the 16-row operand and the columns as N: keys x channels for
 // the scores, channels x keys for the output, because a decode step has few columns (heads of a
@@ -638,13 +638,15 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
   const int seen_all = (int)min(max(len - p.n_tokens + 1 - key0, (int64_t)0), p.chunk_keys);
   const int seen_any = (int)(key1 - key0);
 
-  // m_run: the largest scaled score so far; weights are taken relative to it.  fp16 weights times scales: scales are taken in
-  // units of a power of two above the largest scale of V so far (the same for the warp's columns), so that no product passes 1, and
-  // the accumulators in units of it too.  While every scale is 0, so are the products, in any unit.
+  // m_run: the largest scaled score so far; weights are taken relative to it.  fp16 weights times scales: a channel group's scales,
+  // and its accumulators, are in units of 2^-15 of a power of two above the largest of its scales of V so far (the same for the
+  // warp's columns), so that no product passes 2^15, and those down to 2^-29 of the largest keep all their bits whatever the
+  // scales of the other groups.  Scales below 2^-100 raise no unit (nor does 0: its products are 0 in any).
   float m_run[NT][2], l_run[NT][2], zsum[kG][NT][2], acc[kG][2][NT][4];
-  uint32_t scale_bound = 127u << 7;  // bf16 bits of the unit
-  bool unset = true;                 // no scale but 0 so far
-  float per_unit = 1.f;              // 1 / unit
+  constexpr uint32_t kLeast = 27;  // biased exponent of 2^-100
+  float per_unit[kG];              // 1 / unit; a power of two
+#pragma unroll
+  for (int gr = 0; gr < kG; ++gr) per_unit[gr] = __uint_as_float((269u - kLeast) << 23);
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -740,27 +742,37 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
       }
     }
     // a scale of V above the bound?  (NaN groups do not count: they make their own channels NaN)
-    float rescale = 1.f;  // old unit / new one
+    bool raised = false;
+    float rescale[kG];  // old unit / new one
     if constexpr (!S::kWide) {
-      uint32_t most = 0;
+      auto bound = [&](int gr) { return (269u - (__float_as_uint(per_unit[gr]) >> 23)) << 7; };  // bf16 bits of 2^15 units
+      uint32_t most[kG] = {};
 #pragma unroll
       for (int i = 0; i < kG / 2; ++i) {
         const uint4 w = *reinterpret_cast<const uint4*>(vp + 16 * (lane + 32 * i));
-        most = max(most, max(max(w.x & 0xFFFFu, w.y & 0xFFFFu), max(w.z & 0xFFFFu, w.w & 0xFFFFu)));
+        const uint32_t x[4] = {w.x & 0xFFFFu, w.y & 0xFFFFu, w.z & 0xFFFFu, w.w & 0xFFFFu};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) most[j % kG] = max(most[j % kG], x[j]);
       }
-      if (__any_sync(0xFFFFFFFFu, most > (unset ? 0u : scale_bound))) {
-        most = 0;
+      bool above = false;
+#pragma unroll
+      for (int gr = 0; gr < kG; ++gr) above |= most[gr] > bound(gr);
+      if (__any_sync(0xFFFFFFFFu, above)) {
+        uint32_t mine = 0;  // of group lane % kG
         for (int e = lane; e < kTileKeys * kG; e += 32) {
           const uint32_t w = reinterpret_cast<const uint32_t*>(vp)[e] & 0xFFFFu;
-          most = max(most, w < 0x7F80u ? w : 0u);
+          mine = max(mine, w < 0x7F80u ? w : 0u);
         }
-        most = __reduce_max_sync(0xFFFFFFFFu, most);
-        if (most > (unset ? 0u : scale_bound)) {
-          const uint32_t e = min(max((most >> 7) + 1, 27u), 227u);
-          rescale = unset ? 1.f : ex2(static_cast<float>(static_cast<int>(scale_bound >> 7) - static_cast<int>(e)));
-          scale_bound = e << 7;
-          per_unit = __uint_as_float((254u - e) << 23);
-          unset = false;
+#pragma unroll
+        for (int gr = 0; gr < kG; ++gr) {
+          const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, lane % kG == gr ? mine : 0u);
+          rescale[gr] = 1.f;
+          if (top > bound(gr)) {
+            const float next = __uint_as_float((268u - (top >> 7)) << 23);
+            rescale[gr] = next / per_unit[gr];
+            per_unit[gr] = next;
+            raised = true;
+          }
         }
       }
     }
@@ -799,7 +811,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
         for (int o = KP == 2 ? 2 : 4; o < 32; o <<= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xFFFFFFFFu, top[j], o));
         top[j] *= scale[n][j];
       }
-      if (__any_sync(0xFFFFFFFFu, rescale != 1.f || top[0] > m_run[n][0] || top[1] > m_run[n][1])) {
+      if (__any_sync(0xFFFFFFFFu, raised || top[0] > m_run[n][0] || top[1] > m_run[n][1])) {
         float alpha[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -813,7 +825,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
           zsum[gr][n][0] *= alpha[0];
           zsum[gr][n][1] *= alpha[1];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) acc[gr][i >> 2][n][i & 3] *= alpha[i & 1] * rescale;
+          for (int i = 0; i < 8; ++i) acc[gr][i >> 2][n][i & 3] *= raised ? alpha[i & 1] * rescale[gr] : alpha[i & 1];
         }
       }
     }
@@ -840,7 +852,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
       for (int gr = 0; gr < kG; ++gr) {
         const float sa = bf16_lo(pa[gr]), sb = bf16_lo(pb[gr]);
         const float za = fmaf(8.f, sa, bf16_hi(pa[gr])), zb = fmaf(8.f, sb, bf16_hi(pb[gr]));
-        const float ua = S::kWide ? sa : sa * per_unit, ub = S::kWide ? sb : sb * per_unit;
+        const float ua = S::kWide ? sa : sa * per_unit[gr], ub = S::kWide ? sb : sb * per_unit[gr];
         uint32_t bp[NT][S::kParts][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -934,7 +946,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
           for (int i = 0; i < 4; ++i) o[i] += __shfl_xor_sync(0xFFFFFFFFu, o[i], 2);
         }
         if constexpr (!S::kWide) {
-          const float unit = __uint_as_float(scale_bound << 16);
+          const float unit = __uint_as_float((254u << 23) - __float_as_uint(per_unit[gr]));
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[i] *= unit;
         }

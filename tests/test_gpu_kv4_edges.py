@@ -86,3 +86,79 @@ def test_kv4_decode_of_a_zeroed_cache():
     assert bool(((lse - math.log(200)).abs() <= 2.0 ** -20).all())
     # four heads a kv head; an exponential, a sum and a quotient
     assert bool(((weights[..., :200] - 4 / 200).abs() <= 4 / 200 * 2.0 ** -20).all()) and bool((weights[..., 200:] == 0).all())
+
+
+# ------------------------------------------------------------------------------------------
+# weights times scales in 16 bits
+# ------------------------------------------------------------------------------------------
+def _check_close(q, kv_rows, lens, out, lse=None, weights=None):
+    """As _check_decode, with what 16-bit queries are held to: a weight times a scale is one fp16 number (half a step: 2^-11
+    of it).  The largest of a group's products lies in [2^13, 2^15], so that the smallest fp16 numbers, half a step of which is 2^-25, add at
+    most 2^-25 2^-13 8 = 2^-35 of the group's largest scale for each key (its code is within 8 of the centre)."""
+    for b, n in enumerate(lens.tolist()):
+        (k, _, _), (v, s, m) = (_quantised(x[b, :, :n]) for x in kv_rows)
+        limit = (torch.arange(q.shape[2], device=DEV) + n - q.shape[2] + 1).clamp(min=0)
+        centre, scale = (m + 8 * s).repeat_interleave(32, -1), q.shape[-1] ** -0.5
+        spread = (v - centre).abs()
+        ref, _, _, wide, size = _reference(q[b].double(), k, v, limit, scale, spread)
+        _, _, _, whole, _ = _reference(q[b].double(), k, v, limit, scale, spread + centre.abs())
+        floor = n * 2.0 ** -35 * s.amax(1, keepdim=True).repeat_interleave(32, -1).repeat_interleave(q.shape[1] // k.shape[0], 0)
+        _check(out[b], ref, q.dtype, HALF[torch.float16], wide + floor / HALF[torch.float16],
+               _fp32_share(n, q.shape[-1], 4 * size + 8), whole)
+    _check_decode(q, kv_rows, lens, out, lse, weights)
+
+
+@HEADS
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [65, 3000])
+def test_kv4_decode_holds_fp16_outputs_to_their_type(n, dim, heads):
+    g = _gen(n + dim + heads)
+    k, v = (_randn(g, 1, 1, n, dim, dtype=torch.bfloat16) for _ in range(2))
+    _decode_and_check(_randn(g, 1, heads, 1, dim, dtype=torch.float16), k, v, _check_close)
+
+
+@TYPES16
+@HEADS
+@pytest.mark.parametrize("dim", [64, 128])
+def test_kv4_decode_channel_groups_of_very_different_size(dim, heads, dtype):
+    """A group of large channels takes nothing from the others."""
+    g = _gen(dim + heads)
+    n = 700
+    k, v = (_randn(g, 1, 1, n, dim) for _ in range(2))
+    for big, small in ((2.0 ** 10, 1.0), (8.0, 2.0 ** -10), (2.0 ** 60, 2.0 ** -60)):
+        if dtype == torch.float16 and big > 2.0 ** 15:
+            continue  # an output beyond the type
+        size = torch.full((dim,), small, device=DEV)
+        size[32:64] = big
+        _decode_and_check(_randn(g, 1, heads, 1, dim, dtype=dtype), k.to(torch.bfloat16), (v * size).to(torch.bfloat16), _check_close)
+
+
+@TYPES16
+@pytest.mark.parametrize("heads", [1, 8, 16])
+def test_kv4_decode_small_weights_beside_large_ones(heads, dtype):
+    """Every 64th key has values of zero and nearly all the weight; the others weigh 2^-22 of it each, and the output is theirs."""
+    n, dim = 4096, 64
+    g = _gen(heads)
+    q = torch.full((1, heads, 1, dim), 1.0, device=DEV).to(dtype)
+    k = torch.zeros(1, 1, n, dim, dtype=torch.bfloat16, device=DEV)
+    k[:, :, ::64] = 22 * math.log(2) / math.sqrt(dim)
+    v = _randn(g, 1, 1, 1, dim, dtype=torch.bfloat16).repeat(1, 1, n, 1)
+    v[:, :, ::64] = 0.0
+    _decode_and_check(q, k, v, _check_close)
+
+
+@TYPES16
+def test_kv4_decode_scales_at_the_ends_of_the_range(dtype):
+    """Values around 2^110 and 2^-110 (bf16 outputs hold them; fp16 ones overflow to infinity or vanish)."""
+    from sva_b200 import kernels
+
+    g = _gen(5)
+    q = _randn(g, 1, 3, 1, 64, dtype=dtype)
+    k, v = (_randn(g, 1, 1, 300, 64, dtype=torch.bfloat16) for _ in range(2))
+    for factor in (2.0 ** 110, 2.0 ** -110):
+        w = (v.float() * factor).to(torch.bfloat16)
+        if dtype == torch.bfloat16:
+            _decode_and_check(q, k, w)
+        else:
+            out = kernels.kv4_decode(q, _filled(k, w), max_len=300)
+            assert not bool(out.isnan().any()) and (factor > 1 or bool((out == 0).all()))
