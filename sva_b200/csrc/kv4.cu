@@ -509,6 +509,9 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
   const int64_t key0 = chunk * p.chunk_keys, key1 = min(len, key0 + p.chunk_keys);
   if (key0 >= len && chunk > 0) return;  // the join reads ceil(len / chunk_keys) chunks (at least one)
 
+  // the first key (counted from key0) of a channel group whose value is not finite and which some columns may not see
+  __shared__ int hidden[kDecWarps][kG];
+  if (lane < kG) hidden[warp][lane] = 0x7FFFFFFF;
   unsigned char* ring = smem + 128 + warp * (kStages * S::kTileBytes);
   const uint32_t bar0 = smem_u32(smem) + warp * (8 * kStages);
   if (lane == 0) {
@@ -685,9 +688,18 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
     unsigned char* vp = vc + kC;
     const bool whole = there && l0 + kTileKeys <= seen_all;
     if (!whole) {
-      // parameters of keys that no column sees can be anything: make their values finite
+      // Parameters of keys that no column sees can be anything: make their values finite.  Of keys that only some see, those that
+      // are not finite become 0 too (0 times NaN is NaN) and make NaN of the columns that do see them at the end.
       const int from = there ? max(0, min(kTileKeys, seen_any - l0)) : 0;
-      for (int e = from * kG + lane; e < kTileKeys * kG; e += 32) reinterpret_cast<uint32_t*>(vp)[e] = 0u;
+      for (int e = max(0, min(from, seen_all - l0)) * kG + lane; e < kTileKeys * kG; e += 32) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(vp) + e;
+        if (e >= from * kG) {
+          *w = 0u;
+        } else if ((*w & 0x7F80u) == 0x7F80u || (*w & 0x7F800000u) == 0x7F800000u) {
+          *w = 0u;
+          atomicMin(&hidden[warp][e % kG], l0 + e / kG);
+        }
+      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
     }
@@ -950,7 +962,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[i] *= unit;
         }
-        const float z = zsum[gr][n][j];
+        const float z = limit[n][j] > hidden[warp][gr] ? NAN : zsum[gr][n][j];
         if (!any_failed && (KP == 1 || t < 2))
           *reinterpret_cast<float4*>(w_o + (warp * S::kCols + c) * D + kGroup * gr + 4 * g) =
               make_float4(o[0] + z, o[1] + z, o[2] + z, o[3] + z);

@@ -162,3 +162,36 @@ def test_kv4_decode_scales_at_the_ends_of_the_range(dtype):
         else:
             out = kernels.kv4_decode(q, _filled(k, w), max_len=300)
             assert not bool(out.isnan().any()) and (factor > 1 or bool((out == 0).all()))
+
+
+# ------------------------------------------------------------------------------------------
+# keys that only the later of the new tokens see
+# ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("n, tokens, heads, kv, dim", [(300, 3, 3, 3, 64), (65, 2, 2, 1, 128), (3, 3, 1, 1, 64), (5000, 4, 16, 2, 64),
+                                                        (400, 150, 1, 1, 64), (256, 5, 8, 2, 128)])
+def test_kv4_decode_non_finite_rows_reach_only_the_tokens_that_see_them(n, tokens, heads, kv, dim, dtype):
+    from sva_b200 import kernels
+
+    q, cache, _, lens, rows, longest = _decode_case([n], heads, kv, dim, tokens, dtype, 0, seed=n)
+    want, want_lse = kernels.kv4_decode(q, cache, seq_lens=lens, max_len=longest, want_lse=True)
+    k, v = (x.clone() for x in rows)
+    first = n - tokens + max(1, tokens // 2)  # the first token that sees it, counted in keys
+    v[0, kv - 1, first, 40], v[0, 0, n - 1, 3] = float("inf"), float("nan")
+    start = torch.zeros(1, dtype=torch.int64, device=DEV)
+    kernels.kv4_write(k, v, cache, start)
+    got = kernels.kv4_decode(q, cache, seq_lens=lens, max_len=longest)
+    position = n - tokens + torch.arange(tokens, device=DEV)  # of every token
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    group = heads // kv
+    bad[0, (kv - 1) * group:, :, 32:64] |= (position >= first)[:, None]
+    bad[0, :group, :, :32] |= (position >= n - 1)[:, None]
+    assert torch.equal(got.isnan(), bad) and torch.equal(got[~bad], want[~bad])
+    # a key that is not a number: nothing is left of the rows that see it, the others are as they were
+    k[0, 0, n - 1, 5] = float("nan")
+    kernels.kv4_write(k, rows[1], cache, start)
+    weights = torch.zeros(1, kv, n, device=DEV)
+    got, lse = kernels.kv4_decode(q, cache, seq_lens=lens, max_len=longest, want_lse=True, weights=weights)
+    assert bool(got[0, :group, -1].isnan().all()) and bool(lse[0, :group, -1].isnan().all())
+    assert torch.equal(got[:, :, :-1], want[:, :, :-1]) and torch.equal(lse[:, :, :-1], want_lse[:, :, :-1])
+    assert torch.equal(got[:, group:], want[:, group:]) and bool(weights[:, 1:].isfinite().all())
