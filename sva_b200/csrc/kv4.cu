@@ -675,7 +675,8 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
       rows_next = rows_of(base + 32);
     }
     const int s = it % kStages;
-    if (!mbar_wait(bar0 + 8 * s, (it / kStages) & 1)) {
+    // by vote: what follows is for whole warps
+    if (!__all_sync(0xFFFFFFFFu, mbar_wait(bar0 + 8 * s, (it / kStages) & 1))) {
       failed = true;
       failed_at = it;
       break;

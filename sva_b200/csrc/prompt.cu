@@ -238,6 +238,12 @@ struct TcBars {
   uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3], v_go[3], v_clean[3];
 };
 
+// Bounded wait of a whole warp: true where every lane saw the phase complete.  Lanes that decided apart would part ways before
+// instructions that take the whole warp.
+__device__ __forceinline__ bool warp_wait(const uint64_t& bar, int turn, volatile int* failed) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait_or(smem_u32(&bar), turn & 1, failed)) != 0;
+}
+
 struct PromptTcParams {
   PromptParams p;
   CUtensorMap q, k, v;
@@ -406,7 +412,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
       const uint32_t one = elect_one(), tm = (uint32_t)uniform((int)tmem);
       const int count = uniform(end - first), dirty = uniform(max(0, masked - first));
       const int counts[2] = {uniform(stop[0] - first), uniform(stop[1] - first)};
-      auto wait = [&](const uint64_t& bar, int turn) { return __all_sync(0xFFFFFFFFu, mbar_wait_or(smem_u32(&bar), turn & 1, failed)) != 0; };
+      auto wait = [&](const uint64_t& bar, int turn) { return warp_wait(bar, turn, failed); };
       constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
       constexpr uint32_t kIdescS = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((kTcRows / 8) << 17) | ((kTcRows / 16) << 24);
       constexpr uint32_t kIdescO =
@@ -489,8 +495,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
     for (int j = max(first, masked); j < end; ++j) {
       const int n = j - first, st = n % S::kStages, turn = n / S::kStages;
       // the copy of this very block is under way (v_full's phase could be any before that), then complete
-      if (!mbar_wait_or(smem_u32(&bars.v_go[st]), clean_turn(j) & 1, failed)) break;
-      if (!mbar_wait_or(smem_u32(&bars.v_full[st]), turn & 1, failed)) break;
+      if (!warp_wait(bars.v_go[st], clean_turn(j), failed)) break;
+      if (!warp_wait(bars.v_full[st], turn, failed)) break;
       const int from = max(0, limit_of(tok0) - j * kTcRows), valid = s.len_k - j * kTcRows;
       unsigned char* tile = sv + st * S::kTileBytes;
       for (int e = (from * 8) + (warp - 10) * 32 + lane; e < kTcRows * 8; e += 64) {
@@ -542,7 +548,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
     bool ok = true;
     for (int j = first; j < stop[x]; ++j) {
       const int n = j - first;
-      if (!mbar_wait_or(smem_u32(&bars.s_full[x]), n & 1, failed)) {
+      if (!warp_wait(bars.s_full[x], n, failed)) {
         ok = false;
         break;
       }
@@ -575,7 +581,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
       const bool grew = mx > m + 8.f;
       // O and P are free once the block before has been added.  (P in the place of S: that S is complete says so.)
       if (S::kApart && n > 0) {
-        if (!mbar_wait_or(smem_u32(&bars.pv_done[x]), (n - 1) & 1, failed)) {
+        if (!warp_wait(bars.pv_done[x], n - 1, failed)) {
           ok = false;
           break;
         }
@@ -624,7 +630,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
       mbar_arrive(smem_u32(&bars.p_full[x]));
     }
     const bool any = stop[x] > first;
-    if (ok && any) ok = mbar_wait_or(smem_u32(&bars.pv_done[x]), S::kApart ? (stop[x] - first - 1) & 1 : 0, failed);
+    if (ok && any) ok = warp_wait(bars.pv_done[x], S::kApart ? stop[x] - first - 1 : 0, failed);
     tc_fence_after();
     const int head = h * p.groups + row % p.groups;
     const int64_t qrow = s.q0 + tok;
