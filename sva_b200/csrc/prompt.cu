@@ -236,6 +236,7 @@ struct TcShape {
 struct TcBars {
   uint64_t q_full[2], s_full[2], s_read[2], p_full[2], pv_done[2];
   uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3], v_go[3], v_clean[3];
+  uint64_t mma_end;
 };
 
 // Bounded wait of a whole warp: true where every lane saw the phase complete.  Lanes that decided apart would part ways before
@@ -342,6 +343,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
       mbar_init(smem_u32(&bars.v_go[i]), 1);
       mbar_init(smem_u32(&bars.v_clean[i]), 2);
     }
+    mbar_init(smem_u32(&bars.mma_end), 1);
     mbar_fence_init();
     failed_flag = 0;
     any_bad = 0;
@@ -356,6 +358,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base;
+
+  // the copies that lane 0 of warp 8 has issued: of both K and V below block `issued`, and of K for that block
+  int issued = first;
+  bool k_issued = false;
 
   // registers from the last four warps to the softmax: 2 x 200 + 96 of the 3 x 168 that the CTA was launched with
   if (warp >= 8) {
@@ -375,7 +381,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
                       (int)(s.q0 + tok0 + x * tp.tokens), bar);
       }
       bool ok = true;
-      int issued = first;
       for (int j = first; j < end && ok; ++j) {
         const int n = j - first, st = n % S::kStages, turn = n / S::kStages;
 #pragma unroll
@@ -389,18 +394,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
           for (int c = 0; c < S::kHalves; ++c)
             tma_load_3d(smem_u32((kv ? sv : sk) + st * S::kTileBytes + c * kTcRows * 128), kv ? &tp.v : &tp.k, 64 * c, h,
                         (int)(s.k0 + (int64_t)j * kTcRows), full);
+          k_issued = kv == 0;
           if (kv) issued = j + 1;
           if (kv && j >= masked) mbar_arrive(smem_u32(&bars.v_go[st]));
-        }
-      }
-      if (!ok) {
-        // what is in flight lands before the shared memory goes to another CTA
-        for (int x = 0; x < 2; ++x)
-          if (stop[x] > first) mbar_wait(smem_u32(&bars.q_full[x]), 0);
-        for (int j = max(first, issued - S::kStages); j < min(end, issued + 1); ++j) {
-          const int n = j - first, st = n % S::kStages, turn = n / S::kStages;
-          mbar_wait(smem_u32(&bars.k_full[st]), turn & 1);
-          if (j < issued) mbar_wait(smem_u32(&bars.v_full[st]), turn & 1);
         }
       }
     }
@@ -474,17 +470,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
         if (!ok) break;
         tc_commit(smem_u32(&bars.v_empty[st]), one);
         if (!S::kApart && n + 1 < count) tc_commit(smem_u32(&bars.k_empty[st1]), one);
-      }
-      if (!ok) {
-        // the MMAs issued so far end before the tensor memory is released
-        __shared__ uint64_t drain;
-        if (lane == 0) {
-          mbar_init(smem_u32(&drain), 1);
-          mbar_fence_init();
-        }
-        __syncwarp();
-        tc_commit(smem_u32(&drain), one);
-        mbar_wait(smem_u32(&drain), 0);
       }
     }
     __syncwarp();
@@ -693,6 +678,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
   }
   tc_fence_before();
   __syncthreads();
+  if (*failed) {
+    // Some role gave up: what is in flight lands, and every MMA issued ends, before the shared and the tensor memory go to
+    // another CTA.  (Else the others have waited for all of it.)
+    if (warp == 8 && lane == 0) {
+      for (int x = 0; x < 2; ++x)
+        if (stop[x] > first) mbar_wait(smem_u32(&bars.q_full[x]), 0);
+      for (int j = max(first, issued - S::kStages); j < min(end, issued + 1); ++j) {
+        const int n = j - first, st = n % S::kStages, turn = n / S::kStages;
+        if (j < issued || k_issued) mbar_wait(smem_u32(&bars.k_full[st]), turn & 1);
+        if (j < issued) mbar_wait(smem_u32(&bars.v_full[st]), turn & 1);
+      }
+    } else if (warp == 9) {
+      tc_commit(smem_u32(&bars.mma_end), elect_one());
+      mbar_wait(smem_u32(&bars.mma_end), 0);
+    }
+  }
   if (warp == 9) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
