@@ -1016,9 +1016,10 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Kv4DecPara
   const int tid = threadIdx.x, lane = tid & 31;
   const int join_blocks = p.n_chunks > 1 ? p.n_cols : 0;
   const int64_t l0 = (int64_t)((int)blockIdx.x - join_blocks) * 1024;
-  if (l0 >= len && (int)blockIdx.x >= join_blocks) return;
   __shared__ float part[kJoinThreads];
+  // by every block: the next kernel of the stream starts when these have ended, and the decode kernel must have by then
   pdl_wait();
+  if (l0 >= len && (int)blockIdx.x >= join_blocks) return;
   auto stats = [&](int col, float* top_out, float* l_out) {  // maximum and sum of a column over its chunks
     const int64_t problem = ((int64_t)b * p.c.n_kv + h) * p.col_tiles + col / COLS;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + problem * p.n_chunks * COLS + col % COLS;

@@ -195,3 +195,18 @@ def test_kv4_decode_non_finite_rows_reach_only_the_tokens_that_see_them(n, token
     assert bool(got[0, :group, -1].isnan().all()) and bool(lse[0, :group, -1].isnan().all())
     assert torch.equal(got[:, :, :-1], want[:, :, :-1]) and torch.equal(lse[:, :, :-1], want_lse[:, :, :-1])
     assert torch.equal(got[:, group:], want[:, group:]) and bool(weights[:, 1:].isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_kv4_decode_of_empty_sequences_with_weights(dtype):
+    """Zeros, -inf, and weights as they were, complete when the next kernel of the stream reads them."""
+    from sva_b200 import kernels
+
+    q, cache, _, _, _, _ = _decode_case([300, 300], 4, 2, 64, 1, dtype, 0, seed=2)
+    none = torch.zeros(2, dtype=torch.int64, device=DEV)
+    for max_len in (0, 64, 300):
+        for _ in range(20):
+            weights, out = torch.full((2, 2, 300), 0.25, device=DEV), torch.full_like(q, 7.0)
+            got, lse = kernels.kv4_decode(q, cache, seq_lens=none, max_len=max_len, weights=weights, want_lse=True, out=out)
+            total = got.float().abs().sum() + (lse != -math.inf).sum() + (weights != 0.25).sum()
+            assert float(total) == 0
