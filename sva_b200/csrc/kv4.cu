@@ -118,41 +118,37 @@ __device__ __forceinline__ float element(const Raw<T>& r, int i) {
     return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
 }
 
+// Two differences x - m, not below 0, rounded to odd: the one towards zero, and where that is not exact its last bit set.  A half
+// step (c + 1/2) s has at most 13 bits and a difference near it 24, so such a difference is a half step only where the exact one is.
+__device__ __forceinline__ uint64_t sub2_odd(uint64_t x, uint64_t minus_m) {
+  uint64_t zero, up;
+  asm("add.rz.f32x2 %0, %1, %2;" : "=l"(zero) : "l"(x), "l"(minus_m));
+  asm("add.rp.f32x2 %0, %1, %2;" : "=l"(up) : "l"(x), "l"(minus_m));
+  return zero | (up & 0x0000000100000001ull);
+}
+
 // The nearest code where the group's scale is far from the ends of the fp32 range.  The quotient d * inv is corrected by its
-// remainder, so that one that is a half k + 1/2 comes out as exactly that, and adding 3 * 2^22 rounds it to even.  16-bit inputs:
-// the fp32 difference decides.  fp32 inputs: what the difference lost is added to the remainder.
+// remainder, so that it is the exact quotient of d rounded once: one that is a half k + 1/2 comes out as exactly that and no other
+// does (the next differences' quotients are more than half a unit away), and adding 3 * 2^22 rounds it to even.
 template <typename T>
 __device__ __forceinline__ uint64_t codes16(const Raw<T>& r, float m, float s) {
   float inv;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
   uint32_t w[2] = {0u, 0u};
-  if constexpr (sizeof(T) == 4) {
+  const uint64_t m2 = pack2(-m, -m), s2 = pack2(-s, -s), i2 = pack2(inv, inv);
+  const uint64_t round2 = pack2(12582912.f, 12582912.f);
 #pragma unroll
-    for (int i = 0; i < kWriteChannels; ++i) {
-      const float x = element<T>(r, i), d = x - m, back = d + m;
-      const float lost = (x - back) + (m - (back - d));  // x - m = d + lost
-      const float c = rintf(d * inv);
-      const float rest = fmaf(-c, s, d) + lost, half = 0.5f * s;
-      const bool odd = (static_cast<int>(c) & 1) != 0;
-      const float up = rest > half || (rest == half && odd) ? 1.f : 0.f;
-      const float down = rest < -half || (rest == -half && odd) ? 1.f : 0.f;
-      w[i >> 3] |= static_cast<uint32_t>(static_cast<int>(c + up - down)) << (4 * (i & 7));
-    }
-  } else {
-    const uint64_t m2 = pack2(-m, -m), s2 = pack2(-s, -s), i2 = pack2(inv, inv);
-    const uint64_t round2 = pack2(12582912.f, 12582912.f);
-#pragma unroll
-    for (int i = 0; i < kWriteChannels; i += 2) {
-      const uint64_t d = add2(pack2(element<T>(r, i), element<T>(r, i + 1)), m2);
-      uint64_t q = mul2(d, i2);
-      q = fma2(fma2(q, s2, d), i2, q);
-      q = add2(q, round2);
-      float lo, hi;
-      unpack2(q, lo, hi);
-      // the code is the low bits; each comes in at the top
-      w[i >> 3] = __funnelshift_r(w[i >> 3], __float_as_uint(lo), 4);
-      w[i >> 3] = __funnelshift_r(w[i >> 3], __float_as_uint(hi), 4);
-    }
+  for (int i = 0; i < kWriteChannels; i += 2) {
+    const uint64_t x = pack2(element<T>(r, i), element<T>(r, i + 1));
+    const uint64_t d = sizeof(T) == 4 ? sub2_odd(x, m2) : add2(x, m2);
+    uint64_t q = mul2(d, i2);
+    q = fma2(fma2(q, s2, d), i2, q);
+    q = add2(q, round2);
+    float lo, hi;
+    unpack2(q, lo, hi);
+    // the code is the low bits; each comes in at the top
+    w[i >> 3] = __funnelshift_r(w[i >> 3], __float_as_uint(lo), 4);
+    w[i >> 3] = __funnelshift_r(w[i >> 3], __float_as_uint(hi), 4);
   }
   return static_cast<uint64_t>(w[1]) << 32 | w[0];
 }

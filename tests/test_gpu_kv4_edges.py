@@ -197,6 +197,81 @@ def test_kv4_decode_non_finite_rows_reach_only_the_tokens_that_see_them(n, token
     assert torch.equal(got[:, group:], want[:, group:]) and bool(weights[:, 1:].isfinite().all())
 
 
+# ------------------------------------------------------------------------------------------
+# codes next to half steps
+# ------------------------------------------------------------------------------------------
+def _codes(cache, rows):
+    c = cache.k_codes[0, 0, :rows]
+    return torch.stack([c & 15, c >> 4], -1).flatten(-2)
+
+
+def _exact_codes(x):
+    """Codes in 64 bits: every difference and product here has at most 53 bits, and a quotient that is no half step differs from
+    one by more than 2^-50 of it."""
+    g = x.double().unflatten(-1, (-1, 32))
+    _, s, m = _quantised(x)
+    return ((g - m[..., None]) / s[..., None]).round().flatten(-2).to(torch.uint8)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32], ids=["fp32"])
+def test_kv4_codes_are_the_exact_quotients_nearest(dtype):
+    """Group minima from 1 down to 2^-24 of the step, of both signs; channels on half steps and one or two units beside them,
+    and channels far below the minimum."""
+    from sva_b200 import kernels
+
+    r = torch.Generator().manual_seed(1)
+    n = 4096
+    e = torch.randint(0, 25 if dtype != torch.float16 else 12, (n,), generator=r)
+    s = ((128 + torch.randint(0, 128, (n,), generator=r)) / 128.0).double()
+    m = (128 + torch.randint(0, 128, (n,), generator=r)) / 128.0 * torch.ldexp(torch.ones(n), -e) * (1 - 2 * torch.randint(0, 2, (n,), generator=r))
+    m = m.double()
+    half = torch.randint(0, 15, (n, 32), generator=r) + 0.5
+    x = (m[:, None] + half * s[:, None]).to(dtype)
+    # a minimum below zero also has channels far below it, on either side of a half step's sum
+    tiny = (128 + torch.randint(0, 128, (n, 32), generator=r)) / 128.0 * (1 - 2 * torch.randint(0, 2, (n, 32), generator=r))
+    tiny = torch.ldexp(tiny.double(), -torch.randint(1, 31 if dtype != torch.float16 else 12, (n, 32), generator=r))
+    pick = torch.randint(0, 7, (n, 32), generator=r)
+    bits = torch.int32 if dtype == torch.float32 else torch.int16
+    x = (x.view(bits) + (pick - 2).clamp(-2, 2).to(bits)).view(dtype)
+    x = x.double().nan_to_num(0.0)  # the pattern below that of zero
+    x = torch.where((pick == 6) & (m[:, None] < 0), tiny, x)
+    x = torch.minimum(torch.maximum(x, m[:, None]), m[:, None] + 15 * s[:, None]).to(dtype)
+    x = torch.where(x.double() < m[:, None], m[:, None].to(dtype), x)
+    x[:, 0], x[:, 1] = m.to(dtype), (m + 14.97 * s).to(dtype)
+    x = x.view(1, 1, n // 2, 64).to(DEV)
+    cache = kernels.kv4_empty(1, 1, n // 2, 64)
+    kernels.kv4_write(x, x, cache, torch.zeros(1, dtype=torch.int64, device=DEV))
+    got, want = _codes(cache, n // 2), _exact_codes(x)[0, 0]
+    wrong = (got != want).nonzero()
+    assert len(wrong) == 0, f"{len(wrong)} codes, first {wrong[0].tolist()}"
+
+
+@pytest.mark.parametrize("dtype, minimum, scale, x, code", [
+    (torch.float32, -2.0 ** -23, 1.0, 6.5, 7),
+    (torch.float32, 2.0 ** -23, 1.0, 7.5, 7),
+    (torch.float32, -2.0 ** -26, 1.0, 0.5, 1),
+    (torch.float32, 2.0 ** -26, 1.0, 1.5, 1),
+    (torch.float32, 0.0, 1.0, 6.5, 6),
+    (torch.float32, 0.0, 1.0, 7.5, 8),
+    (torch.float32, 5.5879354e-07, 0.35546875, 4.087891, 11),
+    (torch.float32, -2.0 ** -110, 2.0 ** -109, 2.0 ** -149, 1),
+])
+def test_kv4_codes_of_sums_that_fp32_rounds_to_half_steps(dtype, minimum, scale, x, code):
+    from sva_b200 import kernels
+
+    s = torch.tensor(scale).to(torch.bfloat16).float()
+    m = torch.tensor(minimum).to(torch.bfloat16).float() if scale != 1e31 else -s / 2
+    row = torch.full((64,), x, dtype=torch.float32)
+    row[::32] = m
+    row[1::32] = m + 14.97 * s
+    row = row.to(dtype).to(DEV).expand(1, 1, 1, 64)
+    cache = kernels.kv4_empty(1, 1, 64, 64)
+    kernels.kv4_write(row, row, cache, torch.zeros(1, dtype=torch.int64, device=DEV))
+    assert cache.k_params[0, 0, 0, 0].tolist() == [float(s), float(m)]
+    got = _codes(cache, 1)[0].tolist()
+    assert got[2:32] == [code] * 30 and got[34:] == [code] * 30 and got[0] == 0
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 def test_kv4_decode_of_empty_sequences_with_weights(dtype):
     """Zeros, -inf, and weights as they were, complete when the next kernel of the stream reads them."""
