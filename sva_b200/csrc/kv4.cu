@@ -139,8 +139,7 @@ __device__ __forceinline__ uint64_t codes16(const Raw<T>& r, float m, float s) {
   const uint64_t round2 = pack2(12582912.f, 12582912.f);
 #pragma unroll
   for (int i = 0; i < kWriteChannels; i += 2) {
-    const uint64_t x = pack2(element<T>(r, i), element<T>(r, i + 1));
-    const uint64_t d = sizeof(T) == 4 ? sub2_odd(x, m2) : add2(x, m2);
+    const uint64_t d = sub2_odd(pack2(element<T>(r, i), element<T>(r, i + 1)), m2);
     uint64_t q = mul2(d, i2);
     q = fma2(fma2(q, s2, d), i2, q);
     q = add2(q, round2);
@@ -162,7 +161,10 @@ __device__ __forceinline__ uint64_t codes16_wide(const Raw<T>& r, float m, float
     float x = 0.f;
 #pragma unroll
     for (int j = 0; j < kWriteChannels; ++j) x = j == i ? element<T>(r, j) : x;
-    const double c = rint((static_cast<double>(x) - m) / s);
+    // rounded to odd, as above
+    const double zero = __dsub_rz(x, m), up = __dsub_ru(x, m);
+    const double d = __longlong_as_double(__double_as_longlong(zero) | (__double_as_longlong(up) & 1ll));
+    const double c = rint(d / s);
     w |= static_cast<uint64_t>(fmin(fmax(c, 0.0), 15.0)) << (4 * i);
   }
   return w;

@@ -213,7 +213,7 @@ def _exact_codes(x):
     return ((g - m[..., None]) / s[..., None]).round().flatten(-2).to(torch.uint8)
 
 
-@pytest.mark.parametrize("dtype", [torch.float32], ids=["fp32"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
 def test_kv4_codes_are_the_exact_quotients_nearest(dtype):
     """Group minima from 1 down to 2^-24 of the step, of both signs; channels on half steps and one or two units beside them,
     and channels far below the minimum."""
@@ -254,6 +254,14 @@ def test_kv4_codes_are_the_exact_quotients_nearest(dtype):
     (torch.float32, 0.0, 1.0, 6.5, 6),
     (torch.float32, 0.0, 1.0, 7.5, 8),
     (torch.float32, 5.5879354e-07, 0.35546875, 4.087891, 11),
+    (torch.bfloat16, -1.0, 2.0, 2.0 ** -30, 1),
+    (torch.bfloat16, -1.0, 2.0, -(2.0 ** -30), 0),
+    (torch.bfloat16, -1.0, 2.0, 0.0, 0),
+    (torch.bfloat16, -6.5, 1.0, 2.0 ** -30, 7),
+    (torch.bfloat16, 2.0 ** -30, 1.0, 7.5, 7),
+    (torch.float16, -6.5, 1.0, 2.0 ** -24, 7),
+    (torch.float32, -0.5e31, 1e31, 1e-10, 1),
+    (torch.float32, -0.5e31, 1e31, -1e-10, 0),
     (torch.float32, -2.0 ** -110, 2.0 ** -109, 2.0 ** -149, 1),
 ])
 def test_kv4_codes_of_sums_that_fp32_rounds_to_half_steps(dtype, minimum, scale, x, code):
