@@ -70,9 +70,21 @@ class SVALlamaServingConfig:
     allow_batch: bool = False
     # Not in the reference, whose prompts go through the summon token by token: "exact" computes calls of
     # more than one token with attention over every key (sva_prompt_attention) while the catalog is written as
-    # before, so that decode steps still summon.  Unpadded prompts only (no attention mask); such
-    # calls add nothing to the summon counters.
+    # before, so that decode steps still summon.  Unpadded prompts only (an attention mask may hide later tokens
+    # and nothing else, which costs a host read of the comparison); such calls add nothing to the summon counters.
     prompt_attention: str = "summon"
+
+
+def _only_causal(mask: torch.Tensor, q_len: int, k_len: int) -> bool:
+    """Whether a mask [B or 1, 1, >= q_len, >= k_len] (truth values, or added to the scores) lets query i see exactly the keys
+    0 .. i + k_len - q_len.  Reads one truth value back from the device."""
+    if mask.dim() != 4 or mask.shape[-2] < q_len or mask.shape[-1] < k_len:
+        return False
+    seen = mask[..., :q_len, :k_len]
+    if seen.dtype != torch.bool:
+        seen = seen > -1e4
+    causal = torch.ones(q_len, k_len, dtype=torch.bool, device=mask.device).tril(k_len - q_len)
+    return bool((seen == causal).all())
 
 
 class SVALlamaAttention(nn.Module):
@@ -190,15 +202,17 @@ class SVALlamaAttention(nn.Module):
         return attn_output, None
 
     # ------------------------------------------------------------------------------------
-    def _exact_prompt(self, q_len: int, attention_mask: torch.Tensor | None) -> bool:
-        """Whether this call's tokens attend to every key (serving option ``prompt_attention``)."""
+    def _exact_prompt(self, q_len: int, k_len: int, attention_mask: torch.Tensor | None) -> bool:
+        """Whether this call's tokens attend to every key (serving option ``prompt_attention``).  The host framework hands
+        out causal masks for unpadded prompts too (every prompt of an eager-attention model, chunks behind a growing cache of
+        an sdpa one); a mask that hides anything else, or shows later tokens, is refused."""
         mode = self.serving.prompt_attention
         if mode not in {"summon", "exact"}:
             raise ValueError(f"Unknown prompt_attention {mode!r}; expected 'summon' or 'exact'.")
         if mode == "summon" or q_len == 1:
             return False
-        if attention_mask is not None:
-            raise ValueError("prompt_attention='exact' takes unpadded prompts without an attention mask.")
+        if attention_mask is not None and not _only_causal(attention_mask, q_len, k_len):
+            raise ValueError("prompt_attention='exact' takes unpadded prompts: the attention mask may hide later tokens only.")
         return True
 
     def _prompt_attention(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, k_len: int) -> torch.Tensor:
@@ -229,7 +243,7 @@ class SVALlamaAttention(nn.Module):
         if mode not in {"scan", "inverted", "inverted_static"}:
             raise ValueError(f"Unknown SVA summon_mode: {mode!r}")
         dev = query.device
-        exact = self._exact_prompt(q_len, attention_mask)
+        exact = self._exact_prompt(q_len, k_len, attention_mask)
         keys = key[0]
         values = value[0]
         if keys.stride(-1) != 1:
@@ -346,7 +360,7 @@ class SVALlamaAttention(nn.Module):
         # prefill (not captured): positions and lengths on the host
         first, last = int(pos[0]), int(pos[-1])
         k_len = last + 1
-        exact = self._exact_prompt(q_len, None)
+        exact = self._exact_prompt(q_len, k_len, None)
         kernels.catalog_encode(flat_keys, self._srep[0], self._srep[1], first, k_len - first, flat_low, flat_codes,
                                n_heads=batch * n_heads)
         if exact:
@@ -387,7 +401,7 @@ class SVALlamaAttention(nn.Module):
             key = key.contiguous()
         if value.stride(-1) != 1:
             value = value.contiguous()
-        exact = self._exact_prompt(q_len, attention_mask)
+        exact = self._exact_prompt(q_len, k_len, attention_mask)
         self._key_catalog_batched(key, q_len)
         if exact:
             return self._prompt_attention(query, key, value, k_len)
