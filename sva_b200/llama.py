@@ -189,15 +189,22 @@ class SVALlamaAttention(nn.Module):
         query_states = self.q_proj(hidden_states).view(hidden_shape).transpose(1, 2)
         key_states = self.k_proj(hidden_states).view(hidden_shape).transpose(1, 2)
         value_states = self.v_proj(hidden_states).view(hidden_shape).transpose(1, 2)
+        position_ids = kwargs.get("position_ids")
+        static = isinstance(past_key_values, StaticCache) and position_ids is not None
+        # before the cache takes this call's rows, so that a refused call can be made again
+        q_len = int(hidden_states.shape[1])
+        key_len = q_len if static or attention_mask is None else int(attention_mask.shape[-1])
+        exact = self._exact_prompt(q_len, key_len, None if static else attention_mask)
         cos, sin = position_embeddings
         query_states, key_states = apply_rotary_pos_emb(query_states, key_states, cos, sin)
         if past_key_values is not None:
             key_states, value_states = past_key_values.update(key_states, value_states, self.layer_idx)
-        position_ids = kwargs.get("position_ids")
-        if isinstance(past_key_values, StaticCache) and position_ids is not None:
+        if static:
             attn_output = self.sva_attention_static(query_states, key_states, value_states, position_ids)
         else:
-            attn_output = self.sva_attention(query_states, key_states, value_states, attention_mask)
+            asked = exact and (attention_mask is None or key_len == key_states.shape[2])
+            attn_output = self.sva_attention(query_states, key_states, value_states, attention_mask,
+                                             **({"exact": True} if asked else {}))
         attn_output = attn_output.transpose(1, 2).contiguous().reshape(*input_shape, -1)
         return attn_output, None
 
@@ -229,21 +236,22 @@ class SVALlamaAttention(nn.Module):
         return out.transpose(1, 2)
 
     def sva_attention(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
-                      attention_mask: torch.Tensor | None) -> torch.Tensor:
-        """query [1, H, q, D]; key/value [1, Hkv, L, D] (not repeated) -> [1, H, q, D]."""
+                      attention_mask: torch.Tensor | None, exact: bool = False) -> torch.Tensor:
+        """query [1, H, q, D]; key/value [1, Hkv, L, D] (not repeated) -> [1, H, q, D].  ``exact``: whether
+        ``_exact_prompt`` has been asked and said so; it is asked here otherwise."""
         batch, n_heads, q_len, head_dim = query.shape
         k_len = int(key.shape[2])
         if batch != 1:
             if not self.serving.allow_batch:
                 raise ValueError("SVA Llama adapter currently expects batch size 1.")
-            return self._sva_attention_batched(query, key, value, attention_mask)
+            return self._sva_attention_batched(query, key, value, attention_mask, exact)
         if query.device.type != "cuda":
             raise RuntimeError("The B200 SVA adapter runs on CUDA devices only; move the model to a GPU.")
         mode = self.serving.summon_mode
         if mode not in {"scan", "inverted", "inverted_static"}:
             raise ValueError(f"Unknown SVA summon_mode: {mode!r}")
         dev = query.device
-        exact = self._exact_prompt(q_len, k_len, attention_mask)
+        exact = exact or self._exact_prompt(q_len, k_len, attention_mask)
         keys = key[0]
         values = value[0]
         if keys.stride(-1) != 1:
@@ -383,7 +391,7 @@ class SVALlamaAttention(nn.Module):
 
     # ------------------------------------------------------------------------------------
     def _sva_attention_batched(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
-                               attention_mask: torch.Tensor | None) -> torch.Tensor:
+                               attention_mask: torch.Tensor | None, exact: bool = False) -> torch.Tensor:
         """query [B, H, q, D]; key/value [B, Hkv, L, D] -> [B, H, q, D]: the scan summon of every
         sequence in one call (allow_batch).  Each sequence gets exactly what a batch-1 call of the
         reference would compute for it (sva/llama.py:171-328)."""
@@ -401,7 +409,7 @@ class SVALlamaAttention(nn.Module):
             key = key.contiguous()
         if value.stride(-1) != 1:
             value = value.contiguous()
-        exact = self._exact_prompt(q_len, k_len, attention_mask)
+        exact = exact or self._exact_prompt(q_len, k_len, attention_mask)
         self._key_catalog_batched(key, q_len)
         if exact:
             return self._prompt_attention(query, key, value, k_len)

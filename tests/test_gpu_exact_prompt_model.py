@@ -3,6 +3,8 @@ models' own calls and with the masks that the host framework makes for them."""
 
 from __future__ import annotations
 
+import dataclasses
+
 import pytest
 import torch
 from transformers import DynamicCache, LlamaConfig, LlamaForCausalLM, StaticCache
@@ -88,3 +90,27 @@ def test_masks_that_hide_keys_are_refused(implementation):
     padded[1, :7] = 0
     with torch.no_grad(), pytest.raises(ValueError, match="attention mask"):
         exact(input_ids=_ids(2, 40), attention_mask=padded, use_cache=False)
+
+
+@pytest.mark.parametrize("implementation", ["eager", "sdpa"])
+def test_a_refused_prompt_leaves_the_cache_as_it_was(implementation):
+    plain, exact = _model(implementation, patched=False), _model(implementation, layers=(0,))
+    ids = _ids(1, 60)
+    hole = torch.ones(1, 50, dtype=torch.long, device="cuda")
+    hole[0, 10] = 0
+    cache, other = DynamicCache(config=plain.config), DynamicCache(config=plain.config)
+    with torch.no_grad():
+        exact(input_ids=ids[:, :30], use_cache=True, past_key_values=cache)
+        with pytest.raises(ValueError, match="attention mask"):
+            exact(input_ids=ids[:, 30:50], attention_mask=hole, use_cache=True, past_key_values=cache)
+        assert [cache.get_seq_length(i) for i in range(2)] == [30, 30]
+        got = exact(input_ids=ids[:, 30:50], use_cache=True, past_key_values=cache).logits
+        plain(input_ids=ids[:, :30], use_cache=True, past_key_values=other)
+        torch.testing.assert_close(got, plain(input_ids=ids[:, 30:50], use_cache=True, past_key_values=other).logits, **TOL)
+        attention = exact.model.layers[0].self_attn
+        attention.serving = dataclasses.replace(attention.serving, prompt_attention="everything")
+        for cache in (cache, StaticCache(config=plain.config, max_cache_len=64)):
+            before = int(cache.get_seq_length(0))
+            with pytest.raises(ValueError, match="prompt_attention"):
+                exact(input_ids=ids[:, 50:], use_cache=True, past_key_values=cache)
+            assert int(cache.get_seq_length(0)) == before
