@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
   __shared__ TcBars bars;
   __shared__ uint32_t tmem_base;
   __shared__ int failed_flag, any_bad;
-  __shared__ int bad_from[DP];
+  __shared__ int bad_from[3][DP];  // the first NaN, inf and -inf of a channel that some row may not see
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // heaviest tiles first: later tiles of a sequence see more keys
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
     failed_flag = 0;
     any_bad = 0;
   }
-  for (int d = tid; d < DP; d += kTcThreads) bad_from[d] = 0x7FFFFFFF;
+  for (int d = tid; d < 3 * DP; d += kTcThreads) (&bad_from[0][0])[d] = 0x7FFFFFFF;
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(512)
                  : "memory");
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
   } else if (warp >= 10) {
     // ---- value rows that some row may not see ----
     // 0 times a non-finite value is NaN, so such values become 0 here.  Rows behind the sequence belong to no
-    // one; a non-finite value of the sequence itself makes its channel NaN in the rows that do see it.
+    // one; a non-finite value of the sequence itself is added to its channel at the end in the rows that do see it.
     for (int j = max(first, masked); j < end; ++j) {
       const int n = j - first, st = n % S::kStages, turn = n / S::kStages;
       // the copy of this very block is under way (v_full's phase could be any before that), then complete
@@ -506,8 +506,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
           for (int i = 0; i < 8; ++i) {
             const uint32_t m = 0xFFFFu << (16 * (i & 1));
             if ((w[i >> 1] & (kExp << (16 * (i & 1)))) == (kExp << (16 * (i & 1)))) {
+              const uint32_t u = w[i >> 1] >> (16 * (i & 1)) & 0xFFFFu;
               w[i >> 1] &= ~m;
-              atomicMin(&bad_from[d0 + i], j * kTcRows + r);
+              atomicMin(&bad_from[(u & 0x7FFFu) != kExp ? 0 : 1 + (u >> 15)][d0 + i], j * kTcRows + r);
             }
           }
           any_bad = 1;
@@ -648,8 +649,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
       }
       if (any_bad) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (limit > bad_from[32 * c + i]) o[i] = 0x7FC00000u;
+        for (int i = 0; i < 32; ++i) {
+          float y = __uint_as_float(o[i]);
+          if (limit > bad_from[0][32 * c + i]) y = NAN;
+          if (limit > bad_from[1][32 * c + i]) y += INFINITY;
+          if (limit > bad_from[2][32 * c + i]) y -= INFINITY;
+          o[i] = __float_as_uint(y);
+        }
       }
       if (!whole) {
 #pragma unroll
