@@ -843,12 +843,9 @@ def _rows_span(index: int, t: torch.Tensor, name: str) -> tuple:
     shape, stride, size = t.shape, t.stride(), t.element_size()
     if len(shape) < 3:
         raise ValueError(f"{name} must be [pages, Hkv, page_rows, ...] tensors")
-    if t.is_contiguous():
-        row = stride[2] * size
-    else:
-        row = math.prod(shape[3:]) * size
-        if 0 not in shape and not t[0, 0].is_contiguous():
-            raise ValueError(f"{name} must have contiguous rows")
+    row = math.prod(shape[3:]) * size  # not stride[2], which can be anything for one row a page
+    if not t.is_contiguous() and 0 not in shape and not t[0, 0].is_contiguous():
+        raise ValueError(f"{name} must have contiguous rows")
     page, head, at = stride[0] * size, stride[1] * size, _there(index, t, name)
     within = (shape[1] - 1) * head + shape[2] * row
     return at, at + (shape[0] - 1) * page + within, page, head, row, within

@@ -1,0 +1,20 @@
+"""What the exact-attention wrappers make of shapes and strides, on the CPU: device -1 is where a CPU tensor is."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from sva_b200 import kernels
+
+
+def test_rows_of_one_row_pages_have_their_own_size():
+    """A dimension of one row may have any stride: what is moved is the row, not the stride."""
+    base = torch.zeros(1, 1, 640, 32, dtype=torch.bfloat16)
+    for t in (base[:, :, ::64][:, :, :1], base[:, :, 5::64][:, :, :1], base.as_strided((1, 1, 1, 32), (7, 9, 11, 1))):
+        assert t.is_contiguous() and t.stride(2) != 32
+        at, end, _, _, row, within = kernels._rows_span(-1, t, "rows")
+        assert (at, end - at, row, within) == (t.data_ptr(), 64, 64, 64)
+    two = torch.zeros(3, 2, 64, 4, 2, dtype=torch.bfloat16)
+    at, end, page, head, row, within = kernels._rows_span(-1, two, "rows")
+    assert (end - at, page, head, row, within) == (two.numel() * 2, 2048, 1024, 16, 2048)

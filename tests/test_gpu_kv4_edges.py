@@ -293,3 +293,17 @@ def test_kv4_decode_of_empty_sequences_with_weights(dtype):
             got, lse = kernels.kv4_decode(q, cache, seq_lens=none, max_len=max_len, weights=weights, want_lse=True, out=out)
             total = got.float().abs().sum() + (lse != -math.inf).sum() + (weights != 0.25).sum()
             assert float(total) == 0
+
+
+def test_cache_evict_of_one_row_pages_moves_the_row_alone():
+    from sva_b200 import kernels
+
+    base = _randn(_gen(4), 1, 1, 640, 32, dtype=torch.bfloat16)
+    before, w, n = base.clone(), torch.ones(1, 1, 1, device=DEV), torch.ones(1, dtype=torch.int64, device=DEV)
+    room = torch.full((1, 1, 64, 32), 5.0, dtype=torch.bfloat16, device=DEV)
+    for rows in (base[:, :, ::640], base.as_strided((1, 1, 1, 32), (7, 9, 11, 1))):
+        kernels.cache_evict([rows], w, n, 1, out=[room[:, :, 3:4]], out_weights=torch.zeros(1, 1, 1, device=DEV))
+        assert torch.equal(room[0, 0, 3], base[0, 0, 0]) and bool((room[0, 0, :3] == 5).all()) and bool((room[0, 0, 4:] == 5).all())
+        room[0, 0, 3] = 5.0
+        kernels.cache_evict([rows], w, n, 1)
+        assert torch.equal(base, before)
