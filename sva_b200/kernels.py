@@ -634,8 +634,8 @@ def _page_table(index: int, t: torch.Tensor | None, n_seqs: int, name: str = "pa
     """(pointer, row stride, columns) of a page table, or of none."""
     if t is None:
         return 0, 0, 0
-    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != n_seqs or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name} must be an int32 [{n_seqs}, max_pages] tensor with contiguous rows")
+    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != n_seqs or t.shape[1] < 1 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be an int32 [{n_seqs}, max_pages >= 1] tensor with contiguous rows")
     return _there(index, t, name), t.stride(0), t.shape[1]
 
 

@@ -18,3 +18,15 @@ def test_rows_of_one_row_pages_have_their_own_size():
     two = torch.zeros(3, 2, 64, 4, 2, dtype=torch.bfloat16)
     at, end, page, head, row, within = kernels._rows_span(-1, two, "rows")
     assert (end - at, page, head, row, within) == (two.numel() * 2, 2048, 1024, 16, 2048)
+
+
+def test_page_tables_without_columns_are_refused():
+    """Their data pointer is null, which the C ABI reads as no table at all."""
+    for cols in (0, 1):
+        table = torch.zeros(2, cols, dtype=torch.int32)
+        if cols:
+            assert kernels._page_table(-1, table, 2)[2] == 1
+        else:
+            with pytest.raises(ValueError, match="page_table"):
+                kernels._page_table(-1, table, 2)
+    assert kernels._page_table(-1, None, 2) == (0, 0, 0)
