@@ -639,6 +639,18 @@ def _page_table(index: int, t: torch.Tensor | None, n_seqs: int, name: str = "pa
     return _there(index, t, name), t.stride(0), t.shape[1]
 
 
+def _unfolded(t: torch.Tensor, name: str) -> None:
+    """Refuses a tensor to write to in which two elements may share memory (an expanded dimension, say): the larger of two
+    strides has to span what lies within."""
+    if t.is_contiguous():
+        return
+    span = 1
+    for stride, size in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1):
+        if stride < span:
+            raise ValueError(f"{name} is written, and its elements must not overlap")
+        span += (size - 1) * stride
+
+
 def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, cu_seqlens: torch.Tensor, *,
                      cu_seqlens_k: torch.Tensor | None = None, causal: bool = True, softmax_scale: float | None = None,
                      out: torch.Tensor | None = None, want_lse: bool = False, status: torch.Tensor | None = None):
@@ -677,6 +689,8 @@ def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
         out = torch.empty((n, n_heads, head_dim), dtype=dtype, device=q.device)
     elif out.shape != q.shape or out.dtype != dtype or (head_dim > 1 and out.stride(2) != 1):
         raise ValueError("out must have q's shape and dtype, with contiguous rows")
+    else:
+        _unfolded(out, "out")
     lse = torch.full((n_heads, n), float("-inf"), dtype=torch.float32, device=q.device) if want_lse else None
     a = _pack_prompt(n_seqs, n_heads, n_kv, head_dim, dtype_code(dtype), 1 if causal else 0,
                      head_dim ** -0.5 if softmax_scale is None else softmax_scale, n, nk, q.data_ptr(), qr, qh,
@@ -817,12 +831,15 @@ def kv4_decode(q: torch.Tensor, cache: Kv4Cache, *, seq_lens: torch.Tensor | Non
         out = torch.empty(shape, dtype=q.dtype, device=q.device)
     elif out.shape != shape or out.dtype != q.dtype or out.stride(3) != 1:
         raise ValueError("out must have q's shape and dtype, with contiguous rows")
+    else:
+        _unfolded(out, "out")
     os = out.stride()
     wp = ws = wh = 0
     if weights is not None:
         if (weights.dtype != torch.float32 or weights.dim() != 3 or weights.stride(2) != 1
                 or weights.shape[:2] != (n_seqs, n_kv) or weights.shape[2] < max_len):
             raise ValueError("weights must be float32 [B, Hkv, >= max_len] with contiguous rows")
+        _unfolded(weights, "weights")
         wp, (ws, wh, _) = _there(index, weights, "weights"), weights.stride()
     lse = torch.empty(n_seqs, n_heads, n_tokens, dtype=torch.float32, device=q.device) if want_lse else None
     a = _pack_decode(n_seqs, n_heads, n_tokens, dtype_code(q.dtype), max_len,
@@ -926,12 +943,14 @@ def cache_evict(rows: Sequence[torch.Tensor], weights: torch.Tensor, seq_lens: t
             raise ValueError("rows must agree in their first three dimensions, and so must out")
         if not in_place and (s.dtype != d.dtype or s.shape[3:] != d.shape[3:]):
             raise ValueError("out must have rows of the same shape and dtype")
+        _unfolded(d, "rows" if in_place else "out")
         read.append(one)
         written.append(two)
         packed.append(_pack_row(one[0], two[0], one[4], one[2], one[3], two[2], two[3]))
     n_kv = like[1]
     w = _weights_span(index, weights, "weights", (n_seqs, n_kv))
     ow = w if in_place else _weights_span(index, dst_weights, "out_weights", (n_seqs, n_kv))
+    _unfolded(dst_weights, "weights" if in_place else "out_weights")
     if like_out[1] != n_kv:
         raise ValueError("out must have rows' kv heads")
     if _spans_meet([] if in_place else [*read, w], [*written, ow]):

@@ -30,3 +30,14 @@ def test_page_tables_without_columns_are_refused():
             with pytest.raises(ValueError, match="page_table"):
                 kernels._page_table(-1, table, 2)
     assert kernels._page_table(-1, None, 2) == (0, 0, 0)
+
+
+def test_tensors_to_write_to_must_not_overlap_themselves():
+    base = torch.zeros(4, 6, 8, 16)
+    for fine in (base, base[:, ::2], base.transpose(0, 2), base[1:3, :, 3:, :5], base[:1].expand(1, 6, 8, 16), base[..., :1].expand(4, 6, 8, 1),
+                 base.view(-1).as_strided((2, 2, 100), (100, 200, 1)), base[:0].expand(0, 6, 8, 16)):
+        kernels._unfolded(fine, "out")
+    for bad in (base[:1].expand(4, 6, 8, 16), base[:, :1].expand(4, 6, 8, 16), base.view(-1).as_strided((2, 2, 100), (150, 50, 1)),
+                base.view(-1).as_strided((4, 64), (63, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            kernels._unfolded(bad, "out")

@@ -307,3 +307,34 @@ def test_cache_evict_of_one_row_pages_moves_the_row_alone():
         room[0, 0, 3] = 5.0
         kernels.cache_evict([rows], w, n, 1)
         assert torch.equal(base, before)
+
+
+# ------------------------------------------------------------------------------------------
+# tensors that are written and overlap themselves; sequences without keys
+# ------------------------------------------------------------------------------------------
+def test_written_tensors_that_overlap_themselves_are_refused():
+    from sva_b200 import kernels
+
+    q, cache, _, n, rows, longest = _decode_case([70, 64], 4, 2, 64, 1, torch.bfloat16, 0, seed=1)
+    sums = torch.zeros(2, 2, 200, device=DEV)
+    kw = dict(seq_lens=n, max_len=longest)
+    for weights in (sums[:1].expand(2, 2, 200), sums[:, :1].expand(2, 2, 200), sums.view(-1).as_strided((2, 2, 100), (150, 50, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            kernels.kv4_decode(q, cache, weights=weights, **kw)
+    kernels.kv4_decode(q, cache, weights=sums.view(-1).as_strided((2, 2, 100), (100, 200, 1)), **kw)  # heads apart, sequences within
+    for out in (q[:1].clone().expand(2, 4, 1, 64), q[:, :1].clone().expand(2, 4, 1, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            kernels.kv4_decode(q, cache, out=out, **kw)
+    p, cu = _randn(_gen(1), 9, 4, 64, dtype=torch.bfloat16), torch.tensor([0, 9], device=DEV)
+    for out in (p[:1].clone().expand(9, 4, 64), p[:, :1].clone().expand(9, 4, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            kernels.prompt_attention(p, p, p, cu, out=out)
+    for bad in (lambda: kernels.cache_evict([rows[0][:1].expand(2, 2, 70, 64)], sums, n, 16),
+                lambda: kernels.cache_evict([rows[0][:, :1].expand(2, 2, 70, 64)], sums, n, 16),
+                lambda: kernels.cache_evict([rows[0]], sums[:1].expand(2, 2, 200), n, 16),
+                lambda: kernels.cache_evict([rows[0]], sums, n, 16, out=[rows[1]], out_weights=sums.clone()[:, :1].expand(2, 2, 200)),
+                lambda: kernels.cache_evict([rows[0]], sums, n, 16, out=[rows[1][:1].expand(2, 2, 70, 64)], out_weights=sums.clone())):
+        with pytest.raises(ValueError, match="overlap"):
+            bad()
+    # what is only read may
+    kernels.cache_evict([rows[0][:1].expand(2, 2, 70, 64)], sums[:1].expand(2, 2, 200), n, 16, out=[rows[1]], out_weights=sums.clone())
