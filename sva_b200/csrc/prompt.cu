@@ -210,11 +210,13 @@ __global__ void __launch_bounds__(256) prompt_simt_kernel(const PromptParams p) 
 //   P = exp2(scale log2e S - m) as 16-bit numbers in tensor memory: beside S (D = 64), or over it (D = 128)
 //   O += P V    128 x D x 128, P in tensor memory
 // While one tile is in its softmax the tensor cores work for the other.  The maximum m that P is relative to
-// moves only when a row's maximum grew by more than 2^8 (P stays below 256, well inside fp16), so O is
-// rescaled rarely.
+// moves only when a row's maximum grew by more than 2^8, so O is rescaled rarely.  fp16 weights are 2^7 larger (at most 2^15): those
+// down to 2^-21 of the row's maximum keep all their bits.
 // Measured (device): 8192 tokens, 9 / 3 heads of 64, bf16: 119 us = 652 TFLOP/s of the causal half; 2 x 61 tokens behind 30011
 // keys, 16 / 2 heads of 128: 52 us.  With 64 channels the exponential unit (16 a cycle and SM, 1024 cycles a tile and block
 // against 512 of MMAs) bounds it and is about 76 % busy: a block of both tiles takes about 2700 cycles.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;  // weights are 2^kLift times exp2(scale log2e S - m)
 constexpr int kTcRows = 128;   // rows of a tile, keys of a block
 constexpr int kTcThreads = 384;
 
@@ -591,7 +593,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
           }
         }
       }
-      const float use = m == -INFINITY ? 0.f : m;
+      const float use = m == -INFINITY ? 0.f : m - kLift<T>;
       const uint64_t minus2 = pack2(-use, -use);
       uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
@@ -621,7 +623,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
     const int head = h * p.groups + row % p.groups;
     const int64_t qrow = s.q0 + tok;
     if (!ok && p.status) atomicExch(p.status, SVA_ERR_TIMEOUT);
-    const float use = m == -INFINITY ? 0.f : m;
+    const float use = m == -INFINITY ? 0.f : m - kLift<T>;  // what the weights are relative to
     const bool whole = tp.splits == 1;
     const bool none = limit == 0;
     const float inv = none ? 0.f : 1.f / l;
@@ -629,7 +631,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_tc_kernel(const __grid_c
     if (!whole) {
       const int64_t at = (((int64_t)slot * p.n_kv + h) * tp.splits + split) * 256 + x * 128 + row;
       po = tp.part_o + at * DP;
-      tp.part_ml[2 * at] = m;
+      tp.part_ml[2 * at] = m - kLift<T>;
       tp.part_ml[2 * at + 1] = ok ? l : NAN;
     } else if (live && p.lse) {
       p.lse[head * p.n_rows + qrow] = none ? -INFINITY : (use + log2f(l)) * 0.6931471805599453f;

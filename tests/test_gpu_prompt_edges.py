@@ -1,4 +1,4 @@
-"""Infinite values of prompts reach the rows that see them as what they are."""
+"""Values and weights of prompts at the ends of their ranges: infinities, and weights far below the largest."""
 
 from __future__ import annotations
 
@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_exact_attention import _prompt_case
+from tests.test_gpu_exact_attention import _check_prompt, _prompt_case
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,20 @@ def test_prompt_infinite_values(lens, lens_k, dim, dtype):
         expect[:lq][last >= at[key], :, channel] = value
     assert torch.equal(got.isnan(), expect.isnan())
     assert torch.equal(got.nan_to_num(0.0, math.inf, -math.inf), expect.nan_to_num(0.0, math.inf, -math.inf))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("lens, lens_k, dim", [([700], [700], 64), ([700], [700], 128), ([3, 2], [9000, 2], 64), ([3, 2], [9000, 2], 128)])
+def test_prompt_small_weights_beside_a_large_one(lens, lens_k, dim, dtype):
+    """The first key has values of zero and nearly all the weight; the others weigh 2^-20.5 of it each, and the output is theirs.
+    The bounds are the general ones: half a step of the type for every weight, whatever its size."""
+    from sva_b200 import kernels
+
+    q, k, v, cu, cu_k = _prompt_case(lens, lens_k, 3, 1, dim, dtype, seed=6)
+    q.fill_(1.0)
+    k.zero_()
+    v[1:] = v[1]
+    for at in cu_k[:-1].tolist():
+        k[at], v[at] = 20.5 * math.log(2) / math.sqrt(dim), 0.0
+    out, lse = kernels.prompt_attention(q, k, v, cu, cu_seqlens_k=cu_k, want_lse=True)
+    _check_prompt(q, k, v, cu, cu_k, out, lse)
