@@ -585,11 +585,11 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Kv4Dec
     if constexpr (!S::kWide) {
       big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
-      // the power of two that brings the column's largest element to [1, 2): exact in fp16, but for what lies 2^-14 below the
-      // largest, which is off by at most 2^-25 of it
-      const uint32_t e = min(max(__float_as_uint(big) >> 23, 1u), 253u);
-      const float factor = __uint_as_float((254u - e) << 23);
-      unit = __uint_as_float(e << 23);
+      // the power of two that brings the column's largest element to [2^14, 2^15): exact in fp16, but for what lies 2^-28 below
+      // the largest, which is off by at most 2^-39 of it
+      const uint32_t e = min(max(__float_as_uint(big) >> 23, 15u), 253u);
+      const float factor = __uint_as_float((268u - e) << 23);
+      unit = __uint_as_float((e - 14u) << 23);
 #pragma unroll
       for (int gr = 0; gr < kG; ++gr)
 #pragma unroll

@@ -338,3 +338,17 @@ def test_written_tensors_that_overlap_themselves_are_refused():
             bad()
     # what is only read may
     kernels.cache_evict([rows[0][:1].expand(2, 2, 70, 64)], sums[:1].expand(2, 2, 200), n, 16, out=[rows[1]], out_weights=sums.clone())
+
+
+@TYPES16
+@HEADS
+@pytest.mark.parametrize("dim", [64, 128])
+def test_kv4_decode_query_channels_far_below_the_largest(dim, heads, dtype):
+    """One query channel 2^20 times the others, on keys as much smaller there: the scores are the others'."""
+    g = _gen(dim + heads)
+    n = 500
+    q = _randn(g, 1, heads, 1, dim) * 2.0 ** -6
+    q[..., 0] = 2.0 ** 14
+    k = _randn(g, 1, 1, n, dim) * 2.0 ** 7
+    k[..., :32] *= 2.0 ** -23
+    _decode_and_check(q.to(dtype), k.to(torch.bfloat16), _randn(g, 1, 1, n, dim, dtype=torch.bfloat16), _check_close)
