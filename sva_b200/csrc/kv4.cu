@@ -47,7 +47,9 @@ struct Kv4 {
 // threads a group: one shuffle joins their extremes, and what is worked out once a group is shared by 16
 // channels); channels go two to an fp32x2 instruction, and numbers become integers by adding 3 * 2^22 (a conversion
 // instruction runs at a quarter of the rate).  Reading, a thread has the 8 channels of one code word.  Measured: 8 x 32768 rows of 3 heads
-// of 64 channels, bf16, keys and values: 73 us written (3.6 TB/s, bound by issue: 12 instructions a channel), 53 us read (5.0 TB/s).
+// of 64 channels, bf16, keys and values: 76 us written (3.5 TB/s), 56 us read (4.7 TB/s); fp32: 116 us (4.0 TB/s) and 113 us.  The write is
+// bound by latency: with 5.5 warps a scheduler 55 % of the cycles issue (14 instructions a channel), and of the 9.9 cycles
+// that a warp takes for an instruction it waits 4.1 for the loads and 1.7 for the instruction before.
 
 constexpr int kWriteChannels = 16;
 
@@ -348,9 +350,9 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
 // group), for which a 128-row tcgen05 tile would be empty.  Slot r of a 16-key tile is physical key
 // slot_key(r), which makes the value loads of a warp fall into 32 different banks.
 //
-// Measured (device): 8 x 32768 keys, 9 / 3 heads of 64, bf16: 23.3 us = 2.7 TB/s of the cache's 63 MB; 64 ragged sequences of
-// 1.69 M keys in pages of 256: 130 us = 4.0 TB/s.  Bound by instruction issue: 207 warp instructions for 16 keys of 64 channels,
-// 85 of them on the integer pipe, which takes one every second cycle.
+// Measured (device): 8 x 32768 keys, 9 / 3 heads of 64, bf16: 23.8 us = 2.6 TB/s of the cache's 63 MB; 64 ragged sequences of
+// 1.69 M keys in pages of 256: 134 us = 3.9 TB/s.  Bound by latency: with 3.3 warps a scheduler (128 registers a thread) 55 % of the active cycles
+// issue, and of the 6.0 cycles that a warp takes for an instruction it waits 1.2 for the one before and 1.0 for memory.
 
 constexpr int kDecWarps = 4;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -1173,8 +1175,8 @@ static int plan_decode(const sva_kv4_cache* c, const sva_kv4_decode_args* a, Kv4
   const int64_t tiles_k = std::max<int64_t>(1, (a->max_len + kTileKeys - 1) / kTileKeys);
   int64_t chunks = std::max<int64_t>(1, slots / problems);
   // at least 4 tiles a CTA (one a warp); at most 64 where lengths may differ, so that long sequences spread (64 ragged sequences of
-  // 4096 to 131072 keys: 130 us with 48 or 64, 139 with 32, 143 with 128); one sequence fills the GPU in one wave of equal
-  // chunks (a million keys: 91 us against 103 with chunks of 64 tiles)
+  // 4096 to 131072 keys: 133 us with 48 or 64, 139 with 32, 146 with 128); one sequence fills the GPU in one wave of equal
+  // chunks (a million keys: 90 us against 105 with chunks of 64 tiles)
   int64_t per = (tiles_k + chunks - 1) / chunks;
   per = std::max<int64_t>(per, kDecWarps);
   if (a->seq_lens && a->n_seqs > 1) per = std::min<int64_t>(per, 64);

@@ -68,8 +68,9 @@ __device__ __forceinline__ bool find_tile(const PromptParams& p, int64_t slot, i
 // ---------------------------------------------------------------------------------------
 // One CTA takes 64 queries of one head and walks the keys in tiles of 64 with a running maximum and
 // sum per row; a thread owns 4 rows x 4 keys of the scores and 4 rows x D / 16 channels of the output.
-// Bound by fp32 issue: 4 D flops a (query, key) pair at 2 x 128 lanes a cycle and SM; 8192 tokens of 9 / 3 heads of 64 took
-// 3.1 ms (25 TFLOP/s).
+// Bound by instruction issue (73 % of the cycles), of which FMAs are less than half: the output loop loads its 4 weights and
+// D / 64 vectors and tests a limit a row for every 16 D / 64 of them.  8192 tokens of 9 / 3 heads of 64 take 3.1 ms (25 TFLOP/s, a
+// third of the fp32 rate).
 constexpr int kSimtRows = 64;
 
 template <typename T, int DP>
@@ -212,9 +213,10 @@ __global__ void __launch_bounds__(256) prompt_simt_kernel(const PromptParams p) 
 // While one tile is in its softmax the tensor cores work for the other.  The maximum m that P is relative to
 // moves only when a row's maximum grew by more than 2^8, so O is rescaled rarely.  fp16 weights are 2^7 larger (at most 2^15): those
 // down to 2^-21 of the row's maximum keep all their bits.
-// Measured (device): 8192 tokens, 9 / 3 heads of 64, bf16: 119 us = 652 TFLOP/s of the causal half; 2 x 61 tokens behind 30011
-// keys, 16 / 2 heads of 128: 52 us.  With 64 channels the exponential unit (16 a cycle and SM, 1024 cycles a tile and block
-// against 512 of MMAs) bounds it and is about 76 % busy: a block of both tiles takes about 2700 cycles.
+// Measured (device): 8192 tokens, 9 / 3 heads of 64, bf16: 120 us = 644 TFLOP/s of the causal half; 2 x 61 tokens behind 30011
+// keys, 16 / 2 heads of 128: 53 us.  With 64 channels the exponential unit (16 a cycle and SM, 1024 cycles a tile and block
+// against 512 of MMAs) is the busiest and about 76 % so in the loop, a block of both tiles taking about 2700 cycles; issue is not what
+// bounds it (36 % of the active cycles).
 template <typename T>
 constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;  // weights are 2^kLift times exp2(scale log2e S - m)
 constexpr int kTcRows = 128;   // rows of a tile, keys of a block

@@ -663,7 +663,8 @@ def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     False: all Lk.  A query that sees no key gets zeros; rows behind the last sequence are left as they
     were.  Returns out [N, H, D] (and the log-sum-exp [H, N] fp32 with ``want_lse``).  bf16 and fp16
     rows of D <= 128 channels, a multiple of 8, run on the tensor cores when every stride is a multiple of 16
-    bytes; other calls on the CUDA cores in fp32.  ``status`` (int32 device scalar) receives a timeout flag.
+    bytes, with the softmax weights rounded to the rows' type (sums and maxima stay fp32); other calls on the CUDA cores in fp32.
+    ``out`` may be q itself, and must not overlap keys, values or itself.  ``status`` (int32 device scalar) receives a timeout flag.
     """
     if not q.is_cuda:
         _cuda(q, "q")
@@ -809,9 +810,10 @@ def kv4_decode(q: torch.Tensor, cache: Kv4Cache, *, seq_lens: torch.Tensor | Non
 
     q [B, H, T, D] (contiguous rows).  Sequence b holds ``seq_lens[b]`` keys, the T new ones among them ([B] int64
     on the device; None: ``max_len``), and its token t sees the first seq_lens[b] - T + t + 1.  ``max_len`` (host)
-    bounds the lengths (default: the cache's capacity).  ``weights`` [B, Hkv, >= max_len] fp32: every key's softmax
+    bounds the lengths (default: the cache's capacity), and the work is shared out by it: a bound far above the lengths leaves
+    short sequences to few blocks.  ``weights`` [B, Hkv, >= max_len] fp32: every key's softmax
     weight, summed over the tokens and the heads that share its kv head, is added in place (``cache_evict``
-    goes by these sums).  Returns out [B, H, T, D] (and the log-sum-exp [B, H, T] fp32 with ``want_lse``).
+    goes by these sums); neither they nor ``out`` may overlap themselves.  Returns out [B, H, T, D] (and the log-sum-exp [B, H, T] fp32 with ``want_lse``).
     A token that sees no key gets zeros.
     """
     if not q.is_cuda:

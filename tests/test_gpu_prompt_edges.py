@@ -51,3 +51,14 @@ def test_prompt_small_weights_beside_a_large_one(lens, lens_k, dim, dtype):
         k[at], v[at] = 20.5 * math.log(2) / math.sqrt(dim), 0.0
     out, lse = kernels.prompt_attention(q, k, v, cu, cu_seqlens_k=cu_k, want_lse=True)
     _check_prompt(q, k, v, cu, cu_k, out, lse)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("lens, lens_k", [([300, 1, 70], [300, 1, 70]), ([5, 9], [5000, 9])])
+def test_prompt_output_in_the_place_of_the_queries(lens, lens_k, dtype):
+    from sva_b200 import kernels
+
+    q, k, v, cu, cu_k = _prompt_case(lens, lens_k, 6, 2, 64, dtype, seed=9)
+    want = kernels.prompt_attention(q, k, v, cu, cu_seqlens_k=cu_k)
+    assert kernels.prompt_attention(q, k, v, cu, cu_seqlens_k=cu_k, out=q) is q
+    assert torch.equal(q, want)
